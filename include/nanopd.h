@@ -417,6 +417,131 @@ int npd_add_rms_norm(void* out, void* x, const void* delta, const void* weight, 
 int npd_silu_mul(void* out, const void* gate_up, int64_t rows, int64_t width, int32_t dtype,
                  void* stream);
 
+/*
+ * Attention with changed scores (no reference counterpart: its kernels take a
+ * scale only, PA/csrc/attention/paged_attention_kernel.cu:39-151). Of query row
+ * at position p, head h, and key j of its sequence:
+ *   t = scale * q.k_j
+ *   softcap c > 0:      t = c * tanh(t / c)
+ *   alibi_slopes given: t -= alibi_slopes[h] * |p - j|     (fp32 [num_heads])
+ *   seen(j) = j < context, first <= j, and ((j <= p and (window == 0 or
+ *             p - j < window)) or j < prefix)
+ *   out = sum over seen j of softmax(t)_j v_j; zeros where no key is seen
+ * first: first_keys[row] (packed documents: where the row's one starts; NULL: 0);
+ * prefix: prefix_lens[sequence] (keys that every row of the sequence sees, later
+ * ones and those before the window too; NULL: 0). softcap 0: none; else from
+ * 1e-30 to 1e30. scale positive and finite. window 0: none. Slopes of 0 or more
+ * (a distance penalty), finite.
+ * Keys that a row does not see have no effect on it, whatever the pool holds
+ * there (NaN and infinities too). k_scale / v_scale (fp32 [num_kv_heads], both
+ * or neither): the pool is FP8 (e4m3 bytes, element = e4m3 * scale), as
+ * npd_paged_kv_store_slots_fp8 writes it.
+ * head_dim: a multiple of 8 from 32 to 256 (FP8 pools: of 16); any block size;
+ * any number of query heads per kv head. out, query and caches 16-byte aligned,
+ * strides multiples of 8 elements. Lengths and ids on the device are clamped
+ * into the tables and the pool.
+ *
+ * npd_paged_attention_scored: one token per sequence, at position
+ * seq_lens[s] - 1 of seq_lens[s] keys (first_keys: [num_seqs]).
+ * workspace: ..._workspace_size(...) bytes (window as the call's; has_prefix:
+ * whether prefix_lens is given), 256-byte aligned, NULL when that is 0. Its
+ * contents need no clearing; the counter region at its start is left alone, so a
+ * workspace of npd_paged_attention serves too if it is large enough.
+ */
+int64_t npd_paged_attention_scored_workspace_size(int64_t num_seqs, int64_t num_heads,
+                                                  int64_t num_kv_heads, int64_t head_dim,
+                                                  int64_t block_size, int64_t max_blocks_per_seq,
+                                                  int64_t window, int32_t has_prefix);
+int npd_paged_attention_scored(void* out, const void* query,
+                               const void* key_cache, const void* value_cache,
+                               const int32_t* block_tables, const int32_t* seq_lens,
+                               int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                               int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                               int64_t max_blocks_per_seq, float scale, float softcap,
+                               const float* alibi_slopes, int64_t window,
+                               const int32_t* first_keys, const int32_t* prefix_lens,
+                               const float* k_scale, const float* v_scale,
+                               int64_t q_stride_seq, int64_t q_stride_head,
+                               int64_t out_stride_seq, int64_t out_stride_head,
+                               void* workspace, int64_t workspace_bytes,
+                               int32_t dtype, void* stream);
+
+/*
+ * npd_paged_attention_scored of a batch whose sequences share prefixes (no
+ * reference counterpart; its block manager's fork shares the blocks,
+ * nanoPD/block_manager/block_manager.py:100-105): the same result, each shared
+ * key read once per group. Group g < num_groups: the sequences cu_groups[g] ..
+ * cu_groups[g+1] - 1 (cu_groups: int32 [num_groups + 1], ascending), whose
+ * tables hold the same blocks for their first shared_lens[g] keys (the first
+ * sequence's table is read there). A sequence shorter than that sees its own
+ * keys of them; one outside every group shares nothing. max_shared_len: a
+ * host-known bound on shared_lens, which sets how many workgroups share the
+ * reading (a larger value on the device still gives right results).
+ */
+int64_t npd_paged_attention_shared_workspace_size(int64_t num_seqs, int64_t num_heads,
+                                                  int64_t num_kv_heads, int64_t head_dim,
+                                                  int64_t block_size, int64_t max_blocks_per_seq,
+                                                  int64_t num_groups, int64_t max_shared_len);
+int npd_paged_attention_shared(void* out, const void* query,
+                               const void* key_cache, const void* value_cache,
+                               const int32_t* block_tables, const int32_t* seq_lens,
+                               const int32_t* cu_groups, const int32_t* shared_lens,
+                               int64_t num_seqs, int64_t num_groups, int64_t max_shared_len,
+                               int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                               int64_t num_blocks, int64_t block_size,
+                               int64_t max_blocks_per_seq, float scale, float softcap,
+                               const float* alibi_slopes, int64_t window,
+                               const float* k_scale, const float* v_scale,
+                               int64_t q_stride_seq, int64_t q_stride_head,
+                               int64_t out_stride_seq, int64_t out_stride_head,
+                               void* workspace, int64_t workspace_bytes,
+                               int32_t dtype, void* stream);
+
+/*
+ * The same scores for prompt chunks: rows, cu_seqlens_q, context_lens, max_q_len
+ * and max_context_len as in npd_paged_prefill_attention (row i of sequence s at
+ * position context_lens[s] - q_len + i; rows before position 0 get zeros).
+ * first_keys: [total_q]; prefix_lens: [num_seqs].
+ */
+int64_t npd_paged_prefill_scored_workspace_size(int64_t num_seqs, int64_t total_q,
+                                                int64_t num_heads, int64_t num_kv_heads,
+                                                int64_t head_dim, int64_t max_q_len,
+                                                int64_t max_context_len);
+int npd_paged_prefill_scored(void* out, const void* query,
+                             const void* key_cache, const void* value_cache,
+                             const int32_t* block_tables, const int32_t* cu_seqlens_q,
+                             const int32_t* context_lens,
+                             int64_t num_seqs, int64_t total_q,
+                             int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                             int64_t num_blocks, int64_t block_size,
+                             int64_t max_blocks_per_seq, int64_t max_q_len,
+                             int64_t max_context_len, float scale, float softcap,
+                             const float* alibi_slopes, int64_t window,
+                             const int32_t* first_keys, const int32_t* prefix_lens,
+                             const float* k_scale, const float* v_scale,
+                             int64_t q_stride_token, int64_t q_stride_head,
+                             int64_t out_stride_token, int64_t out_stride_head,
+                             void* workspace, int64_t workspace_bytes,
+                             int32_t dtype, void* stream);
+
+/*
+ * The norms around a block of a layer that norms what the block returns as well
+ * (no reference counterpart):
+ *   d     = delta * rsqrt(mean(delta^2) + eps) * post_weight  (post_weight NULL: delta)
+ *   x_out = residual_scale * x + gate * d      (gate NULL: d), rounded to the dtype
+ *   h     = x_out * rsqrt(mean(x_out^2) + eps) * weight       (h and weight NULL: no h)
+ * per row, fp32 inside. All [rows, width] contiguous (weights [width]), 16-byte
+ * aligned, width a multiple of 8 up to 8192. gate element (r, c) is
+ * gate[r * gate_stride_row + c * gate_stride_col], gate_stride_col 0 or 1: a gate
+ * per column (row stride 0), per row (column stride 0) or per element. x_out may
+ * be x or delta; no other output may overlap an input.
+ */
+int npd_block_norms(void* x_out, void* h, const void* x, const void* delta,
+                    const void* post_weight, const void* weight, const void* gate,
+                    int64_t gate_stride_row, int64_t gate_stride_col,
+                    int64_t rows, int64_t width, float residual_scale, float eps,
+                    int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

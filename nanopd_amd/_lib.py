@@ -57,6 +57,18 @@ SIGNATURES = {
     "npd_qk_norm_rope_store_fp8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                                   _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                                   _F, _I32, _P]),
+    "npd_paged_attention_scored_workspace_size": (_I64, [_I64] * 7 + [_I32]),
+    "npd_paged_attention_scored": (ctypes.c_int, [_P] * 6 + [_I64] * 7 + [_F, _F, _P, _I64, _P, _P,
+                                                                         _P, _P] + [_I64] * 4 +
+                                   [_P, _I64, _I32, _P]),
+    "npd_paged_attention_shared_workspace_size": (_I64, [_I64] * 8),
+    "npd_paged_attention_shared": (ctypes.c_int, [_P] * 8 + [_I64] * 9 + [_F, _F, _P, _I64, _P, _P] +
+                                   [_I64] * 4 + [_P, _I64, _I32, _P]),
+    "npd_paged_prefill_scored_workspace_size": (_I64, [_I64] * 7),
+    "npd_paged_prefill_scored": (ctypes.c_int, [_P] * 7 + [_I64] * 10 + [_F, _F, _P, _I64, _P, _P, _P,
+                                                                        _P] + [_I64] * 4 +
+                                 [_P, _I64, _I32, _P]),
+    "npd_block_norms": (ctypes.c_int, [_P] * 7 + [_I64] * 4 + [_F, _F, _I32, _P]),
     "npd_add_rms_norm": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _F, _I32, _P]),
     "npd_silu_mul": (ctypes.c_int, [_P, _P, _I64, _I64, _I32, _P]),
     "npd_pack_metadata": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P,

@@ -12,6 +12,11 @@ plus the ops the MI355X path adds:
 * :func:`paged_prefill_attention` -- varlen chunked prefill over the paged prefix
 * :func:`copy_blocks` -- copy-on-write block copy
 * :func:`qk_norm_rope_store` -- Qwen3 q/k RMSNorm + RoPE + paged K/V store, fused
+* :func:`paged_attention_scored`, :func:`paged_prefill_attention_scored` --
+  decode and prefill whose scores are capped, pay for distance, end at a window,
+  or are masked by document or prefix
+* :func:`paged_attention_shared` -- decode of a batch that shares prefixes
+* :func:`block_norms` -- the norms before and after a block, gate and residual
 * :func:`pack_metadata` -- ragged-batch metadata built on the GPU
 
 Every op validates its arguments here (``RuntimeError``, as ``TORCH_CHECK``
@@ -33,6 +38,9 @@ __all__ = [
     "paged_kv_store", "paged_kv_store_slots", "paged_attention_forward",
     "paged_prefill_attention", "copy_blocks", "pack_metadata", "BatchMetadata",
     "attention_workspace_bytes", "prefill_workspace_bytes", "qk_norm_rope_store",
+    "paged_attention_scored", "paged_prefill_attention_scored", "paged_attention_shared",
+    "scored_workspace_bytes", "prefill_scored_workspace_bytes", "shared_workspace_bytes",
+    "block_norms",
 ]
 
 _DTYPES = {torch.float16: _lib.NPD_DTYPE_F16, torch.bfloat16: _lib.NPD_DTYPE_BF16}
@@ -707,6 +715,265 @@ def qk_norm_rope_store(q_out: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
               qkv.stride(0), q_out.stride(0), float(eps), code, _stream(dev))
 
 
+# ---------------------------------------------------------------------------
+# Attention with changed scores
+# ---------------------------------------------------------------------------
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """The library call with the tensors' device current: kernels launch on the
+    stream of the device that is."""
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _stream(dev))
+
+
+def _score_rule(what, out, query, key_cache, value_cache, block_tables, scale, block_size,
+                max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale, lens):
+    """Checks that the scored ops share. lens: (tensor, name, least length) of the
+    int32 vectors, None where not given. Returns the cache sizes, the element code
+    and the pointers of the score arguments."""
+    if not (isinstance(query, torch.Tensor) and query.is_cuda):
+        _fail("query is must be on CUDA")
+    if not (query.dim() == 3):
+        _fail(f"{what}: query must be [tokens, num_heads, head_size]")
+    fp8 = k_scale is not None or v_scale is not None
+    if fp8:
+        _fp8_cache_checks(key_cache, value_cache, k_scale, v_scale)
+    else:
+        _cache_checks(key_cache, value_cache)
+    dev = query.device
+    _int32(block_tables, "block_tables")
+    given = [x for x in lens if x[0] is not None]
+    for t, nm, n in given:
+        _int32(t, nm)
+        if not (t.dim() == 1 and t.numel() >= n and t.is_contiguous()):
+            _fail(f"{nm} must be a contiguous int32 vector of at least {n}")
+    _same_device(dev, out, key_cache, value_cache, block_tables, *(x[0] for x in given))
+    if fp8:
+        _same_device(dev, k_scale, v_scale)
+    h, d = query.size(1), query.size(2)
+    num_blocks, kvh, bs, cd = key_cache.shape
+    if not (cd == d):
+        _fail(f"head_dim {d} does not match cache head_dim {cd}")
+    if not (int(block_size) == bs):
+        _fail(f"block_size {block_size} does not match cache block size {bs}")
+    if not (kvh > 0 and h > 0 and h % kvh == 0):
+        _fail(f"num_heads {h} is not a multiple of num_kv_heads {kvh}")
+    if not (out.shape == query.shape and out.dtype == query.dtype):
+        _fail("out must match query")
+    if not (fp8 or query.dtype == key_cache.dtype):
+        _fail("query/cache dtype mismatch")
+    code = _dtype_code(query, what)
+    mb = int(max_num_blocks_per_seq)
+    if not (block_tables.dim() == 2 and block_tables.size(1) == mb and block_tables.is_contiguous()):
+        _fail("block_tables must be a contiguous [num_seqs, max_num_blocks_per_seq] tensor")
+    if not (query.stride(2) == 1 and out.stride(2) == 1):
+        _fail("head_dim must be the contiguous dim")
+    slopes = 0
+    if alibi_slopes is not None:
+        if not (isinstance(alibi_slopes, torch.Tensor) and alibi_slopes.dtype == torch.float32
+                and alibi_slopes.shape == (h,) and alibi_slopes.is_contiguous()):
+            _fail("alibi_slopes must be a contiguous float32 [num_heads] tensor")
+        _same_device(dev, alibi_slopes)
+        slopes = alibi_slopes.data_ptr()
+    rule = (float(scale), float(softcap), slopes, int(window))
+    scales = (k_scale.data_ptr(), v_scale.data_ptr()) if fp8 else (0, 0)
+    return (num_blocks, kvh, bs, d, mb), code, rule, scales
+
+
+def _scored_workspace(workspace, need: int, dev: torch.device):
+    """(the workspace, its pointer, its bytes): the caller's, or one of this call
+    from torch's allocator, which orders its reuse by stream and leaves it to a
+    graph that is being captured."""
+    if need <= 0:
+        return None, 0, 0
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    else:
+        _same_device(dev, workspace)
+        if not (workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need):
+            _fail(f"workspace of {need} bytes needed")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+@functools.lru_cache(maxsize=1024)
+def _scored_ws(name: str, *sizes: int) -> int:
+    return int(getattr(_lib.load(), name)(*sizes))
+
+
+def scored_workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                           block_size: int, max_num_blocks_per_seq: int, window: int = 0,
+                           prefix: bool = False) -> int:
+    """Bytes that :func:`paged_attention_scored` needs (prefix: with prefix_lens)."""
+    return _scored_ws("npd_paged_attention_scored_workspace_size", int(num_seqs), int(num_heads),
+                      int(num_kv_heads), int(head_dim), int(block_size),
+                      int(max_num_blocks_per_seq), int(window), int(bool(prefix)))
+
+
+def shared_workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                           block_size: int, max_num_blocks_per_seq: int, num_groups: int,
+                           max_shared_len: int) -> int:
+    """Bytes that :func:`paged_attention_shared` needs."""
+    return _scored_ws("npd_paged_attention_shared_workspace_size", int(num_seqs), int(num_heads),
+                      int(num_kv_heads), int(head_dim), int(block_size),
+                      int(max_num_blocks_per_seq), int(num_groups), int(max_shared_len))
+
+
+def prefill_scored_workspace_bytes(num_seqs: int, total_q: int, num_heads: int, num_kv_heads: int,
+                                   head_dim: int, max_q_len: int, max_context_len: int) -> int:
+    """Bytes that :func:`paged_prefill_attention_scored` needs."""
+    return _scored_ws("npd_paged_prefill_scored_workspace_size", int(num_seqs), int(total_q),
+                      int(num_heads), int(num_kv_heads), int(head_dim), int(max_q_len),
+                      int(max_context_len))
+
+
+def paged_attention_scored(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor,
+                           value_cache: torch.Tensor, block_tables: torch.Tensor,
+                           seq_lens: torch.Tensor, scale: float, block_size: int,
+                           max_num_blocks_per_seq: int, softcap: float = 0.0,
+                           alibi_slopes: torch.Tensor | None = None, window: int = 0,
+                           first_keys: torch.Tensor | None = None,
+                           prefix_lens: torch.Tensor | None = None,
+                           k_scale: torch.Tensor | None = None,
+                           v_scale: torch.Tensor | None = None,
+                           workspace: torch.Tensor | None = None) -> None:
+    """:func:`paged_attention_forward` with changed scores (no reference
+    counterpart: its kernel takes a scale only,
+    PA/csrc/attention/paged_attention_kernel.cu:39-151).
+
+    The token of sequence s sits at p = seq_lens[s] - 1. Its score of key j is
+    ``t = scale * q.k_j``; with ``softcap`` c > 0 ``t = c * tanh(t / c)``; with
+    ``alibi_slopes`` (float32 [num_heads], 0 or more) then ``t -= slope * |p - j|``.
+    It sees key j where ``first_keys[s] <= j`` and either ``p - j < window``
+    (0: no window) or ``j < prefix_lens[s]`` (first keys that stay visible behind
+    a window). Both are int32 [num_seqs], 0 when not given. A token that sees
+    nothing gets zeros; keys not seen have no effect, whatever the pool holds.
+    ``k_scale`` / ``v_scale`` (float32 [num_kv_heads]): an FP8 pool.
+    head_dim a multiple of 8 from 32 to 256 (FP8: of 16), any block size and
+    group. ``workspace``: at least :func:`scored_workspace_bytes` bytes (its
+    contents do not matter) in place of one allocated per call.
+    """
+    s = query.size(0) if isinstance(query, torch.Tensor) and query.dim() == 3 else 0
+    (num_blocks, kvh, bs, d, mb), code, rule, scales = _score_rule(
+        "paged_attention_scored", out, query, key_cache, value_cache, block_tables, scale,
+        block_size, max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale,
+        ((seq_lens, "seq_lens", s), (first_keys, "first_keys", s), (prefix_lens, "prefix_lens", s)))
+    _int32(seq_lens, "seq_lens")
+    if not (block_tables.size(0) >= s):
+        _fail("block_tables must be [num_seqs, max_num_blocks_per_seq]")
+    if s == 0:
+        return
+    h, dev = query.size(1), query.device
+    need = _scored_ws("npd_paged_attention_scored_workspace_size", s, h, kvh, d, bs, mb, int(window),
+                      int(prefix_lens is not None))
+    ws, ws_ptr, ws_bytes = _scored_workspace(workspace, need, dev)
+    _call_on(dev, "npd_paged_attention_scored", out.data_ptr(), query.data_ptr(),
+             key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+             seq_lens.data_ptr(), s, h, kvh, d, num_blocks, bs, mb, *rule,
+             0 if first_keys is None else first_keys.data_ptr(),
+             0 if prefix_lens is None else prefix_lens.data_ptr(), *scales, query.stride(0),
+             query.stride(1), out.stride(0), out.stride(1), ws_ptr, ws_bytes, code)
+
+
+def paged_attention_shared(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor,
+                           value_cache: torch.Tensor, block_tables: torch.Tensor,
+                           seq_lens: torch.Tensor, scale: float, block_size: int,
+                           max_num_blocks_per_seq: int, cu_groups: torch.Tensor,
+                           shared_lens: torch.Tensor, max_shared_len: int, softcap: float = 0.0,
+                           alibi_slopes: torch.Tensor | None = None, window: int = 0,
+                           k_scale: torch.Tensor | None = None,
+                           v_scale: torch.Tensor | None = None,
+                           workspace: torch.Tensor | None = None) -> None:
+    """:func:`paged_attention_scored` of a batch whose sequences share prefixes
+    (forks of one prompt, nanoPD/block_manager/block_manager.py:100-105): the same
+    result, with each shared key read once per group instead of once per sequence.
+
+    Sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int32 [num_groups + 1],
+    ascending) form group g; their tables hold the same blocks for the first
+    shared_lens[g] keys (int32 [num_groups]). seq_lens and block_tables are whole,
+    as without groups. A sequence outside every group shares nothing; one shorter
+    than its group's shared keys sees its own. ``max_shared_len``: a host-side
+    bound on shared_lens (it sets how many workgroups share the reading).
+    ``workspace``: at least :func:`shared_workspace_bytes` bytes.
+    """
+    s = query.size(0) if isinstance(query, torch.Tensor) and query.dim() == 3 else 0
+    _int32(cu_groups, "cu_groups")
+    ng = cu_groups.numel() - 1
+    if not (cu_groups.dim() == 1 and ng >= 1):
+        _fail("cu_groups must be a contiguous int32 [num_groups + 1] vector of one group at least")
+    (num_blocks, kvh, bs, d, mb), code, rule, scales = _score_rule(
+        "paged_attention_shared", out, query, key_cache, value_cache, block_tables, scale,
+        block_size, max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale,
+        ((seq_lens, "seq_lens", s), (cu_groups, "cu_groups", ng + 1), (shared_lens, "shared_lens", ng)))
+    _int32(seq_lens, "seq_lens")
+    _int32(shared_lens, "shared_lens")
+    if not (block_tables.size(0) >= s):
+        _fail("block_tables must be [num_seqs, max_num_blocks_per_seq]")
+    if s == 0:
+        return
+    h, dev = query.size(1), query.device
+    mshared = min(int(max_shared_len), mb * bs)
+    need = _scored_ws("npd_paged_attention_shared_workspace_size", s, h, kvh, d, bs, mb, ng, mshared)
+    ws, ws_ptr, ws_bytes = _scored_workspace(workspace, need, dev)
+    _call_on(dev, "npd_paged_attention_shared", out.data_ptr(), query.data_ptr(),
+             key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+             seq_lens.data_ptr(), cu_groups.data_ptr(), shared_lens.data_ptr(), s, ng, mshared, h,
+             kvh, d, num_blocks, bs, mb, *rule, *scales, query.stride(0), query.stride(1),
+             out.stride(0), out.stride(1), ws_ptr, ws_bytes, code)
+
+
+def paged_prefill_attention_scored(out: torch.Tensor, query: torch.Tensor,
+                                   key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                   block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                                   context_lens: torch.Tensor, scale: float, block_size: int,
+                                   max_num_blocks_per_seq: int, max_q_len: int,
+                                   max_context_len: int | None = None, softcap: float = 0.0,
+                                   alibi_slopes: torch.Tensor | None = None, window: int = 0,
+                                   first_keys: torch.Tensor | None = None,
+                                   prefix_lens: torch.Tensor | None = None,
+                                   k_scale: torch.Tensor | None = None,
+                                   v_scale: torch.Tensor | None = None,
+                                   workspace: torch.Tensor | None = None) -> None:
+    """:func:`paged_prefill_attention` with the scores of
+    :func:`paged_attention_scored`. Row i of sequence s sits at
+    p = context_lens[s] - q_len + i and sees key j < context_lens[s] where
+    ``first_keys[row] <= j`` and either ``j <= p`` and ``p - j < window`` (0: no
+    window), or ``j < prefix_lens[s]``. first_keys: int32 [total_q], where the
+    row's document starts in packed documents; prefix_lens: int32 [num_seqs], keys
+    that every row of the sequence sees, also from before them. Rows past
+    cu_seqlens_q[-1] are left as they were. ``workspace``: at least
+    :func:`prefill_scored_workspace_bytes` bytes (contents do not matter).
+    """
+    tq = query.size(0) if isinstance(query, torch.Tensor) and query.dim() == 3 else 0
+    _int32(cu_seqlens_q, "cu_seqlens_q")
+    ns = cu_seqlens_q.numel() - 1
+    if not (cu_seqlens_q.dim() == 1 and ns >= 0):
+        _fail("cu_seqlens_q must be a contiguous [num_seqs + 1] tensor")
+    (num_blocks, kvh, bs, d, mb), code, rule, scales = _score_rule(
+        "paged_prefill_attention_scored", out, query, key_cache, value_cache, block_tables, scale,
+        block_size, max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale,
+        ((cu_seqlens_q, "cu_seqlens_q", ns + 1), (context_lens, "context_lens", ns),
+         (first_keys, "first_keys", tq), (prefix_lens, "prefix_lens", ns)))
+    _int32(context_lens, "context_lens")
+    if not (block_tables.size(0) >= ns):
+        _fail("block_tables must be [num_seqs, max_num_blocks_per_seq]")
+    if ns == 0 or tq == 0:
+        return
+    h, dev = query.size(1), query.device
+    mq = min(int(max_q_len), tq)
+    mctx = mb * bs if max_context_len is None else min(int(max_context_len), mb * bs)
+    need = _scored_ws("npd_paged_prefill_scored_workspace_size", ns, tq, h, kvh, d, mq, mctx)
+    ws, ws_ptr, ws_bytes = _scored_workspace(workspace, need, dev)
+    _call_on(dev, "npd_paged_prefill_scored", out.data_ptr(), query.data_ptr(),
+             key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+             cu_seqlens_q.data_ptr(), context_lens.data_ptr(), ns, tq, h, kvh, d, num_blocks, bs,
+             mb, mq, mctx, *rule, 0 if first_keys is None else first_keys.data_ptr(),
+             0 if prefix_lens is None else prefix_lens.data_ptr(), *scales, query.stride(0),
+             query.stride(1), out.stride(0), out.stride(1), ws_ptr, ws_bytes, code)
+
+
 def _rows_16(*ts: torch.Tensor) -> bool:
     """Contiguous 2-byte tensors of one dtype and one GPU that start on 16 bytes,
     with whole 16-byte rows, none empty, none to record a gradient for."""
@@ -740,6 +1007,67 @@ def add_rms_norm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tens
     if delta is not None:
         x += delta
     return torch.nn.functional.rms_norm(x, (x.size(-1),), weight, eps)
+
+
+def block_norms(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor | None,
+                weight: torch.Tensor | None, eps: float, gate: torch.Tensor | None = None,
+                residual_scale: float = 1.0,
+                x_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """The norms around a block, for layers that norm what a block returns as well
+    (:func:`add_rms_norm` is the form without)::
+
+        d = rms_norm(delta) * post_weight            (None: delta itself)
+        x = residual_scale * x + gate * d            (None: d), rounded to the dtype
+        return rms_norm(x) * weight                  (None: returns None)
+
+    over the last dim of 2-D tensors. The new x is left in ``x``, or in ``x_out``
+    if given (which may be delta). gate broadcasts against x: [width], [rows, 1] or
+    [rows, width]. 2-byte CUDA tensors of up to 8192 columns run as one launch with
+    fp32 inside; others, and calls that record a gradient, as torch operations,
+    which take a new x_out only through x (they refuse what does not fit)."""
+    ts = [t for t in (delta, post_weight, weight, x_out) if t is not None]
+    if (x.dim() == 2 and x.size(1) <= 8192 and delta.shape == x.shape and _rows_16(x, *ts)
+            and (post_weight is None or post_weight.shape == x.shape[1:])
+            and (weight is None or weight.shape == x.shape[1:])
+            and (x_out is None or x_out.shape == x.shape)):
+        strides = (0, 0) if gate is None else _gate_strides(gate, x)
+        if strides is not None:
+            dst = x if x_out is None else x_out
+            h = None if weight is None else torch.empty_like(x)
+            _call_on(x.device, "npd_block_norms", dst.data_ptr(), 0 if h is None else h.data_ptr(),
+                     x.data_ptr(), delta.data_ptr(),
+                     0 if post_weight is None else post_weight.data_ptr(),
+                     0 if weight is None else weight.data_ptr(),
+                     0 if gate is None else gate.data_ptr(), *strides, x.size(0), x.size(1),
+                     float(residual_scale), float(eps), _DTYPES[x.dtype])
+            return h
+    norm, cols = torch.nn.functional.rms_norm, (x.size(-1),)
+    d = delta.float()
+    if post_weight is not None:
+        d = norm(d, cols, post_weight.float(), eps)
+    if gate is not None:
+        d = gate.float() * d
+    y = (residual_scale * x.float() + d).to(x.dtype)
+    if not (y.shape == x.shape):
+        _fail(f"block_norms: delta and gate do not fit x of {list(x.shape)}")
+    (x if x_out is None else x_out).copy_(y)
+    return None if weight is None else norm(y.float(), cols, weight.float(), eps).to(x.dtype)
+
+
+def _gate_strides(gate: torch.Tensor, x: torch.Tensor) -> tuple[int, int] | None:
+    """Element strides (row, column) of a gate that the kernel reads as it is: one
+    per column, per row or per element of x, on x's device and of its type."""
+    if (gate.dtype != x.dtype or gate.get_device() != x.get_device() or gate.dim() not in (1, 2)
+            or (torch.is_grad_enabled() and gate.requires_grad)):
+        return None
+    r, c = (gate.size(0) if gate.dim() == 2 else 1), gate.size(-1)
+    if r not in (1, x.size(0)) or c not in (1, x.size(1)):
+        return None
+    row = gate.stride(0) if gate.dim() == 2 and r > 1 else 0
+    col = gate.stride(-1) if c > 1 else 0
+    if col == 1 and (gate.data_ptr() & 15 or row & 7):
+        return None
+    return (row, col) if col in (0, 1) else None
 
 
 def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:
