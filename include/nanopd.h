@@ -475,8 +475,7 @@ int npd_paged_attention_scored(void* out, const void* query,
  * tables hold the same blocks for their first shared_lens[g] keys (the first
  * sequence's table is read there). A sequence shorter than that sees its own
  * keys of them; one outside every group shares nothing. max_shared_len: a
- * host-known bound on shared_lens, which sets how many workgroups share the
- * reading (a larger value on the device still gives right results).
+ * host-known bound on shared_lens (keys past it are read per sequence).
  */
 int64_t npd_paged_attention_shared_workspace_size(int64_t num_seqs, int64_t num_heads,
                                                   int64_t num_kv_heads, int64_t head_dim,

@@ -33,7 +33,10 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoRef = 3.402823466e38f;   // exponent offset of a row without a reference
 constexpr int kTileRows = 128;              // rows of a workgroup of the rows kernel
-constexpr int kStepKeys = 64;               // keys per step of the rows kernel
+// ... and how many of them run at once on a compute unit at (padded) head dim d
+__host__ __device__ constexpr int rows_per_cu(int64_t d) { return d > 128 ? 1 : d > 64 ? 2 : 3; }
+constexpr int kStepKeys = 32;               // keys per step of the rows kernel
+constexpr int kListTiles = 512;             // most tiles per kv head that are cut into parts
 constexpr int kUnitHeads = 16;              // most heads of a stream unit (MFMA columns)
 
 // One call. Rows are (token, head) pairs of a kv head's G query heads.
@@ -52,17 +55,18 @@ struct Args {
   const float* v_scale;
   const int32_t* cu_groups;       // shared prefixes: sequences of group g are
   const int32_t* shared_lens;     // cu_groups[g] .. cu_groups[g + 1] - 1
-  float* tile_o;                  // partials of the rows kernel [tile][kv head][part][row][D]
+  float* tile_o;                  // partials of the rows kernel [item][kv head][row][D]
   float* tile_ml;                 // their (m, l)
-  int32_t* tile_parts;            // [tile][kv head] parts written (0: no key)
+  int32_t* tile_items;            // [tile][kv head]: first item and parts
   float* unit_o;                  // partials of the stream kernel [seq][head][part][D]
   float* unit_ml;
-  int num_seqs, num_groups, total_q;
+  int num_seqs, num_groups, total_q, max_shared;
   int num_heads, num_kv_heads, group, head_dim;
   int block_size, bs_shift, num_blocks, max_bps;   // bs_shift < 0: no power of two
   int tiles;                      // rows kernel: tiles of all sequences or groups
   int tiles_max;                  // ... chunks: most tiles of one sequence
-  int tile_splits;                // ... most parts of a tile
+  int items, room;                // ... items per kv head, and those that run at once
+  bool list;                      // ... tiles are cut into parts (else one item each)
   int unit_splits;                // stream kernel: most parts of a unit
   int subs, sub_heads;            // stream kernel: units per kv head, heads of a unit
   int window;                     // 0: none
@@ -122,7 +126,7 @@ __device__ __forceinline__ Group group_at(const Args& a, int g) {
   Group r;
   r.seq0 = clampi(a.cu_groups[g], 0, a.num_seqs);
   r.seqs = clampi(a.cu_groups[g + 1], r.seq0, a.num_seqs) - r.seq0;
-  r.shared = clampi(a.shared_lens[g], 0, a.max_bps * a.block_size);
+  r.shared = clampi(a.shared_lens[g], 0, a.max_shared);
   r.tile0 = 0;
   return r;
 }

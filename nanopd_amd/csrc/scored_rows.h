@@ -2,11 +2,10 @@
 // read the same keys -- prompt chunks, and the tokens of a group of sequences
 // over their shared prefix.
 //
-// Workgroup: 4 waves = 128 flattened (token, head) rows of one kv head, and a
-// part of the keys they see. K/V tiles of 64 keys load straight into LDS
+// Workgroup: 4 waves of 32 flattened (token, head) rows of one kv head, and a part
+// of the keys they see. K/V tiles of 32 keys load straight into LDS
 // (global_load_lds, 16 bytes per lane; FP8 bytes through registers, converted
-// exactly), two tiles of each, the next one loading under the step. Per step a
-// wave forms
+// exactly), the next ones under the step. Per step a wave forms
 //   S^T = K . Q^T     (32x32x16 MFMA, its 32 query rows in registers),
 //   P   = 2^(t - m)   (scored.h; masks only in steps that some row sees in part),
 //   O^T += V^T . P^T  (V through transposing LDS reads).
@@ -14,14 +13,20 @@
 // maximum is taken in the usual step. Steps run from the last key back: the
 // newest keys come first, which with a distance term hold the largest scores.
 //
+// What bounds it: the issue of exponentials and reciprocals. One wave issues an
+// exponential every 24 cycles and any other vector instruction every 8 (measured),
+// a SIMD one every 8 and 4: it takes three waves per SIMD to fill it, so registers
+// and LDS are held to three workgroups per compute unit (two at head dims above
+// 128, four up to 64), which run unsynchronised, one's MFMAs under another's
+// exponentials.
+//
 // Masked keys: P is 0 by selection, but 0 times an infinity or NaN in V is NaN,
 // and rows of a tile do not see the same keys. So a row whose result is not
 // finite is computed again, key by key over what it sees (redo_row); a finite
 // result had no such product.
 //
-// Bound: the MFMAs and the exponentials share the issue of a SIMD. Two
-// workgroups per compute unit run unsynchronised (head dims up to 128), one's
-// MFMAs under the other's exponentials.
+// Parts: a launch that does not fill the chip several times over cuts its tiles
+// into parts of about equal steps (rows_list), from the lengths on the device.
 #pragma once
 
 #include "scored.h"
@@ -30,7 +35,10 @@ namespace npd {
 namespace scored {
 
 constexpr int kThreads = 256;
-constexpr int kListBlocks = 2048;    // pool blocks listed in LDS at a time (8 KB)
+constexpr int kListEntries = 1024;   // pool blocks listed in LDS at a time (4 KB)
+constexpr int kAhead = 4;            // LDS operand reads ahead of their MFMA
+constexpr int kMinPartSteps = 8;     // shortest part of a tile
+constexpr int kListSlots = kListTiles / 64;
 
 // LDS position of 16-byte chunk c of tile row r is c ^ swz(r): rows are D * 2
 // bytes apart without padding (direct loads write 1 KB runs), and the swizzle
@@ -48,16 +56,19 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(lds), "v"(p) : "memory", "m0");
 }
-// Every load and LDS access of this wave is done; then the workgroup's barrier.
-__device__ __forceinline__ void wait_all_and_barrier() {
+// At most N direct loads of this wave are in flight, its LDS accesses are done;
+// then the workgroup's barrier.
+template <int N>
+__device__ __forceinline__ void wait_and_barrier() {
   __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
+constexpr int kWaitVm0 = 0x0f70;            // s_waitcnt vmcnt(0), the other counters free
 
 // When a row's reference moves. bf16: it sits kBias above the maximum it was
 // taken from, and a P of 2 or more (bit 14 of a half) asks for a new one. fp16
-// keeps it at the maximum, and asks where a lane's 32 P of a step come to 2^8 or
+// keeps it at the maximum, and asks where a lane's 16 P of a step come to 2^8 or
 // more: one of them then passed it by kMove.
 template <class TT>
 struct Bound;
@@ -72,98 +83,244 @@ struct Bound<F16> {
 
 __device__ __forceinline__ int wave_min_i(int x) { return -wave_max_i(-x); }
 
-// The item of a workgroup: rows f0 .. of a tile, and where they come from.
+// The item of a workgroup: a tile of rows and part `part` of `cut`.
 struct Item {
-  int s;        // block table row
-  int row0;     // first token row of q / out (chunks: of the chunk; groups: sequence)
-  int rows;     // flattened rows of the chunk or group
-  int t;        // tile of them
-  int limit;    // keys at or past it belong to no row here (context, or shared keys)
-  int ctx;      // chunks: context; groups: unused
-  int qlen;     // chunks: tokens
+  int s;         // block table row
+  int row0;      // first token row of q / out
+  int tokens;    // tokens of the chunk, or sequences of the group
+  int t;         // tile of them
+  int limit;     // keys at or past it belong to no row here (context, or shared keys)
+  int tile;      // index of the tile among all
+  int part, cut;
 };
 
-template <class TT, int D, bool kF8, bool kCap, bool kBias>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+// x / d for 0 <= x < 2^21, 0 < d: the fp32 estimate is off by at most one.
+__device__ __forceinline__ int small_div(int x, int d) {
+  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+  const int r = x - q * d;
+  return q + (r >= d ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+
+// The steps of a part so that all parts fit `room` at once: the mean load, and
+// more while the parts' round-ups pass the room (not where whole tiles do).
+// count(target) gives the parts of all tiles.
+template <class F>
+__device__ __forceinline__ int part_steps(int64_t total, int tiles, int room, F count) {
+  int target = (int)((total + room - 1) / room);
+  target = target < kMinPartSteps ? kMinPartSteps : target;
+  if (tiles < room)
+    for (int k = 0; k < 12 && count(target) > room; ++k) target += 1 + target / 16;
+  return target;
+}
+
+// Item `id` of a kv head, by one wave: the tiles' parts one after another. Chunks:
+// the last tiles first; a tile's steps are those of its causal range and window.
+// Groups: every tile of a group has the steps of its shared keys. false: none.
+__device__ __forceinline__ bool rows_list(const Args& a, int id, int lane, Item& it) {
+  const int G = a.group, cap = a.max_bps * a.block_size;
+  if (!a.cu_seqlens_q) {
+    int64_t total = 0;
+    int tiles = 0;
+    auto at = [&](int g, Group& r, int& nt, int& n) {
+      r = Group{0, 0, 0, 0};
+      nt = n = 0;
+      if (g < a.num_groups) {
+        r = group_at(a, g);
+        nt = (r.seqs * G + kTileRows - 1) / kTileRows;
+        n = (r.shared + kStepKeys - 1) / kStepKeys;
+      }
+    };
+    Group r;
+    int nt, n;
+    for (int g0 = 0; g0 < a.num_groups; g0 += 64) {
+      at(g0 + lane, r, nt, n);
+      // in pieces of 2^15 steps, so that the wave sums stay in 31 bits
+      const int sum = wave_sum_i(nt * (n >> 6)), low = wave_sum_i(nt * (n & 63));
+      total += (int64_t)sum * 64 + low;
+      tiles += wave_sum_i(n > 0 ? nt : 0);
+    }
+    auto parts = [](int nn, int target) { return (nn + target - 1) / target; };
+    const int target = part_steps(total, tiles, a.room, [&](int tg) {
+      int c = 0;
+      for (int g0 = 0; g0 < a.num_groups; g0 += 64) {
+        if (a.num_groups > 64) at(g0 + lane, r, nt, n);
+        c += wave_sum_i(nt * parts(n, tg));
+      }
+      return c;
+    });
+    int base = 0, tbase = 0;
+    for (int g0 = 0; g0 < a.num_groups; g0 += 64) {
+      if (a.num_groups > 64) at(g0 + lane, r, nt, n);
+      const int cut = parts(n, target);
+      const int ic = wave_scan_i(nt * cut), tc = wave_scan_i(nt);
+      const int i0 = base + ic - nt * cut;
+      const uint64_t m = __ballot(id >= i0 && id < base + ic);
+      if (m != 0) {
+        const int sel = __builtin_ctzll(m);
+        auto of = [&](int x) { return __builtin_amdgcn_readlane(x, sel); };
+        it.cut = of(cut);
+        const int e = id - of(i0);
+        it.t = e / it.cut;
+        it.part = e - it.t * it.cut;
+        it.s = it.row0 = of(r.seq0);
+        it.tokens = of(r.seqs);
+        it.limit = of(r.shared);
+        it.tile = tbase + of(tc) - of(nt) + it.t;
+        if (it.tile >= a.tiles) it.cut = 0;   // groups that overlap
+        return true;
+      }
+      base += __builtin_amdgcn_readlane(ic, 63);
+      tbase += __builtin_amdgcn_readlane(tc, 63);
+    }
+    return false;
+  }
+  // chunks: slot (k, lane) is tile i = last - (64 k + lane) of num_seqs * tiles_max
+  const int all = a.num_seqs * a.tiles_max;
+  auto chunk = [&](int sq, int& q0, int& ql, int& cx) {
+    q0 = clampi(a.cu_seqlens_q[sq], 0, a.total_q);
+    ql = clampi(a.cu_seqlens_q[sq + 1], q0, a.total_q) - q0;
+    cx = clampi(a.seq_lens[sq], 0, cap);
+  };
+  int n[kListSlots];
+  int total = 0, tiles = 0;
+#pragma unroll
+  for (int k = 0; k < kListSlots; ++k) {
+    n[k] = 0;
+    const int i = all - 1 - (64 * k + lane);
+    if (64 * k < all && i >= 0) {
+      const int sq = small_div(i, a.tiles_max), t = i - sq * a.tiles_max;
+      int q0, ql, cx;
+      chunk(sq, q0, ql, cx);
+      if (t * kTileRows < ql * G) {
+        const int p0 = cx - ql + small_div(t * kTileRows, G);
+        const int p1 = cx - ql + min(ql, small_div((t + 1) * kTileRows + G - 1, G));
+        const int lo = a.window > 0 && p0 - a.window + 1 > 0 ? p0 - a.window + 1 : 0;
+        n[k] = max(1, (max(p1, 0) + kStepKeys - 1) / kStepKeys - lo / kStepKeys);
+      }
+    }
+    total += n[k];
+    tiles += n[k] > 0 ? 1 : 0;
+  }
+  total = wave_sum_i(total);
+  tiles = wave_sum_i(tiles);
+  auto parts = [&](int k, int tg) { return small_div(n[k] + tg - 1, tg); };
+  const int target = part_steps(total, tiles, a.room, [&](int tg) {
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < kListSlots; ++k)
+      if (64 * k < all) c += parts(k, tg);
+    return wave_sum_i(c);
+  });
+  int base = 0, i = -1;
+#pragma unroll
+  for (int k = 0; k < kListSlots; ++k)
+    if (64 * k < all && i < 0) {
+      const int cut = parts(k, target);
+      const int ic = wave_scan_i(cut);
+      const uint64_t m = __ballot(id >= base + ic - cut && id < base + ic);
+      if (m != 0) {
+        const int sel = __builtin_ctzll(m);
+        it.cut = __builtin_amdgcn_readlane(cut, sel);
+        it.part = id - (base + __builtin_amdgcn_readlane(ic, sel) - it.cut);
+        i = all - 1 - (64 * k + sel);
+      }
+      base += __builtin_amdgcn_readlane(ic, 63);
+    }
+  if (i < 0) return false;
+  it.s = i / a.tiles_max;
+  it.t = i - it.s * a.tiles_max;
+  chunk(it.s, it.row0, it.tokens, it.limit);
+  it.tile = (int)((int64_t)it.row0 * G / kTileRows) + it.s + it.t;
+  return true;
+}
+
+// kCapped: no cap, a plain one, or one past kCapPlain.
+enum Capped { kNoCap, kPlainCap, kWideCap };
+template <class TT, int D, bool kF8, Capped kCapped, bool kBias>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(rows_per_cu(D), rows_per_cu(D))))
 void rows_kernel(Args a) {
   constexpr int KT = kStepKeys;
+  constexpr int TR = kTileRows;
+  constexpr int kBufs = D > 128 ? 2 : 3;    // K and V tiles in LDS
   constexpr int RB = 2 * D;                 // bytes of a tile row
   constexpr int TB = KT * RB;               // bytes of a tile
   constexpr int NI = TB / 4096;             // 1 KB loads per wave and tile
-  constexpr int NC = D / 16, NS = KT / 32, KB = KT / 16, DB = D / 32;
+  constexpr int NC = D / 16, KB = KT / 16, DB = D / 32;
   constexpr int EB = kF8 ? 1 : 2;
-  __shared__ __attribute__((aligned(1024))) char s_k[2 * TB];
-  __shared__ __attribute__((aligned(1024))) char s_v[2 * TB];
-  __shared__ int s_row[kListBlocks];
+  constexpr bool kCap = kCapped != kNoCap;
+  static_assert(KT == 32 && NI >= 1, "one 32-key block per step");
+  __shared__ __attribute__((aligned(1024))) char s_k[kBufs * TB];
+  __shared__ __attribute__((aligned(1024))) char s_v[kBufs * TB];
+  __shared__ int s_row[kListEntries];
   __shared__ int s_red[4][4];
+  __shared__ Item s_item;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hf = lane >> 5, c32 = lane & 31;
   const int G = a.group, d = a.head_dim, bs = a.block_size;
   const int cap_keys = a.max_bps * bs;
+  auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
-  // ---- the item: kv head fastest (with 8 of them each XCD's L2 serves one),
-  // the last tile of a chunk first (it sees the most keys)
-  int id = blockIdx.x;
-  const int kh = id % a.num_kv_heads;
-  id /= a.num_kv_heads;
+  // ---- the item: kv head fastest (with 8 of them each XCD's L2 serves one)
+  const int kh = (int)blockIdx.x % a.num_kv_heads, id = (int)blockIdx.x / a.num_kv_heads;
   Item it;
-  int part;
-  int64_t tile;      // of all sequences or groups
-  if (a.cu_seqlens_q) {
-    const int per = a.tiles_max * a.num_seqs;
-    part = id / per;
-    id -= part * per;
+  if (a.list) {
+    if (wave == 0) {
+      Item w{};
+      rows_list(a, id, lane, w);    // cut 0: no item
+      if (lane == 0) s_item = w;
+    }
+    __syncthreads();
+    it = Item{uni(s_item.s), uni(s_item.row0), uni(s_item.tokens), uni(s_item.t),
+              uni(s_item.limit), uni(s_item.tile), uni(s_item.part), uni(s_item.cut)};
+    if (it.cut == 0) return;
+  } else {
+    // whole tiles of chunks, the last of a sequence first (it sees the most keys)
     it.s = id / a.tiles_max;
     it.t = a.tiles_max - 1 - (id - it.s * a.tiles_max);
-    const int q0 = clampi(a.cu_seqlens_q[it.s], 0, a.total_q);
-    it.qlen = clampi(a.cu_seqlens_q[it.s + 1], q0, a.total_q) - q0;
-    it.ctx = clampi(a.seq_lens[it.s], 0, cap_keys);
-    it.row0 = q0;
-    it.rows = it.qlen * G;
-    it.limit = it.ctx;
-    tile = (int64_t)q0 * G / kTileRows + it.s + it.t;
-  } else {
-    part = id / a.tiles;
-    tile = id - part * a.tiles;
-    Group g;
-    if (!find_group<false>(a, (int)tile, lane, g)) return;
-    it.s = it.row0 = g.seq0;
-    it.qlen = g.seqs;
-    it.rows = g.seqs * G;
-    it.t = (int)tile - g.tile0;
-    it.limit = g.shared;
-    it.ctx = 0;
+    it.row0 = clampi(a.cu_seqlens_q[it.s], 0, a.total_q);
+    it.tokens = clampi(a.cu_seqlens_q[it.s + 1], it.row0, a.total_q) - it.row0;
+    it.limit = clampi(a.seq_lens[it.s], 0, cap_keys);
+    it.part = 0;
+    it.cut = 1;
+    it.tile = 0;
+    if ((int64_t)it.t * TR >= (int64_t)it.tokens * G) return;
   }
-  if (it.t * kTileRows >= it.rows) return;
+  const int frows = it.tokens * G;
 
   // ---- this lane's row (past the last: a copy of it, not stored)
-  const int f0 = it.t * kTileRows + wave * 32;
-  const bool row_ok = f0 + c32 < it.rows;
-  const int f = row_ok ? f0 + c32 : it.rows - 1;
+  const int f0 = it.t * TR + wave * 32;
+  const bool row_ok = f0 + c32 < frows;
+  const int f = row_ok ? f0 + c32 : frows - 1;
   const int tok = f / G;
   const int h = kh * G + (f - tok * G);
   const int qrow = it.row0 + tok;
-  int pos, ctx = it.ctx;
+  int pos, ctx;
   if (a.cu_seqlens_q) {
-    pos = ctx - it.qlen + tok;
+    ctx = it.limit;
+    pos = ctx - it.tokens + tok;
   } else {
     ctx = clampi(a.seq_lens[qrow], 0, cap_keys);
     pos = ctx - 1;
   }
   Keys see = row_keys(pos, ctx, a.first_keys ? a.first_keys[qrow] : 0,
                       a.prefix_lens ? a.prefix_lens[it.s] : 0, a.window);
-  see.hi = see.hi < it.limit ? see.hi : it.limit;
-  see.pre = see.pre < it.limit ? see.pre : it.limit;
+  see.hi = min(see.hi, it.limit);
+  see.pre = min(see.pre, it.limit);
   if (see.lo >= see.hi) see.lo = see.hi = 0;          // empty ranges are [0, 0)
   if (see.first >= see.pre) see.first = see.pre = 0;
 
-  // ---- the wave's and the workgroup's ranges: near [lo, hi), far [first, pre)
-  constexpr int kFar = 0x7fffffff;
-  const int w_lo = wave_min_i(see.hi > 0 ? see.lo : kFar), w_hi = wave_max_i(see.hi);
-  const int w_first = wave_min_i(see.pre > 0 ? see.first : kFar), w_pre = wave_max_i(see.pre);
-  // keys that every row of the wave sees: [w_lo1, w_hi0) and [w_first1, w_pre0)
-  const int w_lo1 = wave_max_i(see.lo), w_hi0 = wave_min_i(see.hi);
+  // ---- ranges: near [lo, hi), far [first, pre); of the wave (none where it has no
+  // row to store) and of the workgroup the keys that some row sees, and of the wave
+  // those that every row sees
+  constexpr int kFarKey = 0x7fffffff;
+  const bool idle = f0 >= frows;
+  const int w_lo = idle ? kFarKey : wave_min_i(see.hi > 0 ? see.lo : kFarKey);
+  const int w_hi = idle ? 0 : wave_max_i(see.hi);
+  const int w_first = idle ? kFarKey : wave_min_i(see.pre > 0 ? see.first : kFarKey);
+  const int w_pre = idle ? 0 : wave_max_i(see.pre);
+  // (a wave without a row masks nothing: its results go nowhere)
+  const int w_lo1 = idle ? 0 : wave_max_i(see.lo), w_hi0 = idle ? kFarKey : wave_min_i(see.hi);
   const int w_first1 = wave_max_i(see.first), w_pre0 = wave_min_i(see.pre);
   if (lane == 0) {
     s_red[0][wave] = w_lo;
@@ -172,11 +329,9 @@ void rows_kernel(Args a) {
     s_red[3][wave] = w_pre;
   }
   __syncthreads();
-  auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  const int nlo = uni(min(min(s_red[0][0], s_red[0][1]), min(s_red[0][2], s_red[0][3])));
-  const int nhi = uni(max(max(s_red[1][0], s_red[1][1]), max(s_red[1][2], s_red[1][3])));
-  const int flo = uni(min(min(s_red[2][0], s_red[2][1]), min(s_red[2][2], s_red[2][3])));
-  const int fhi = uni(max(max(s_red[3][0], s_red[3][1]), max(s_red[3][2], s_red[3][3])));
+  auto least = [&](const int (&x)[4]) { return uni(min(min(x[0], x[1]), min(x[2], x[3]))); };
+  auto most = [&](const int (&x)[4]) { return uni(max(max(x[0], x[1]), max(x[2], x[3]))); };
+  const int nlo = least(s_red[0]), nhi = most(s_red[1]), flo = least(s_red[2]), fhi = most(s_red[3]);
   // step ranges [fs0, fs1) and [ns0, ns1), one range where they meet; key
   // bounds of each for the loads
   int ns0 = nhi > 0 ? nlo / KT : 0, ns1 = (nhi + KT - 1) / KT;
@@ -190,29 +345,24 @@ void rows_kernel(Args a) {
     fs0 = fs1 = 0;
   }
   const int nfar = fs1 - fs0, nsteps = nfar + ns1 - ns0;
-  int nsp = 0;
-  if (nsteps > 0) {
-    nsp = (nsteps + 3) / 4;      // a part has four steps at least
-    nsp = nsp < a.tile_splits ? nsp : a.tile_splits;
+  const bool merged = a.cu_groups || it.cut > 1;
+  if (a.list && it.part == 0 && tid == 0) {
+    a.tile_items[2 * (it.tile * a.num_kv_heads + kh)] = id;
+    a.tile_items[2 * (it.tile * a.num_kv_heads + kh) + 1] = it.cut;
   }
-  const bool merged = a.cu_groups || nsp > 1;
-  if (a.tile_parts && part == 0 && tid == 0)
-    a.tile_parts[tile * a.num_kv_heads + kh] = nsp;
-  uint16_t* op = a.out + (int64_t)qrow * a.out_stride_token + (int64_t)h * a.out_stride_head;
-  if (part >= nsp) {
-    if (part == 0 && !a.cu_groups && row_ok)   // no key at all: zero rows
-      for (int e = hf * 4; e < d; e += 8) *reinterpret_cast<u32x2*>(op + e) = u32x2{0, 0};
-    return;
-  }
-  const int base = nsteps / nsp, rem = nsteps - base * nsp;
-  const int st0 = part * base + min(part, rem), st1 = st0 + base + (part < rem ? 1 : 0);
+  const int base = nsteps / it.cut, rem = nsteps - base * it.cut;
+  const int st0 = it.part * base + min(it.part, rem), st1 = st0 + base + (it.part < rem ? 1 : 0);
 
   // ---- queries as B operands: qb[c] = Q[row][16c + 8 hf ..], zeros past the row
-  const uint16_t* qp = a.q + (int64_t)qrow * a.q_stride_token + (int64_t)h * a.q_stride_head;
+  uint16_t* op = a.out + (int64_t)qrow * a.out_stride_token + (int64_t)h * a.out_stride_head;
   u32x4 qb[NC];
+  {
+    const uint16_t* qp = a.q + (int64_t)qrow * a.q_stride_token + (int64_t)h * a.q_stride_head;
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-    qb[c] = c * 16 + hf * 8 < d ? *reinterpret_cast<const u32x4*>(qp + c * 16 + hf * 8) : u32x4{0, 0, 0, 0};
+    for (int c = 0; c < NC; ++c)
+      qb[c] = c * 16 + hf * 8 < d ? *reinterpret_cast<const u32x4*>(qp + c * 16 + hf * 8)
+                                  : u32x4{0, 0, 0, 0};
+  }
   const float kscale = kF8 ? a.k_scale[kh] : 1.f;
   const float c2 = a.scale_log2 * kscale, cin = a.cap_in * kscale, capA = a.cap_log2;
   const float slope = kBias ? a.slopes[h] * kLog2e : 0.f;
@@ -222,55 +372,55 @@ void rows_kernel(Args a) {
   const int64_t rowb = (int64_t)d * EB;
   const int last16 = (int)(rowb / 16) - 1;
   constexpr int LROW = kF8 ? D / 16 : RB / 16;         // lanes per row
-  constexpr int NR = kF8 ? KT * D / (kThreads * 16) : NI;
-  static_assert(NR >= 1, "tile shape");
-  int lrow[NR], lcol[NR];
+  constexpr int NR = kF8 ? (KT * LROW + kThreads - 1) / kThreads : NI;
+  constexpr bool kSome = kF8 && KT * LROW < kThreads;  // some threads load
+  // load e of a lane: tile row lrow0 + e * kRows, column lcol[e]
+  constexpr int kRows = kF8 ? kThreads / LROW : 1024 / RB;
+  const int lrow0 = kF8 ? tid / LROW : (wave * NI * 1024 + lane * 16) / RB;
+  uint32_t lcol[NR];
 #pragma unroll
   for (int e = 0; e < NR; ++e) {
-    int c;
-    if (kF8) {
-      lrow[e] = (tid + kThreads * e) / LROW;
-      c = (tid + kThreads * e) % LROW;
-    } else {
-      const int o = (wave * NI + e) * 1024 + lane * 16;
-      lrow[e] = o / RB;
-      c = (o % RB / 16) ^ swz<D>(lrow[e]);
-    }
-    lcol[e] = (c < last16 ? c : last16) * 16;
+    const int c = kF8 ? tid % LROW : (lane * 16 % RB / 16) ^ swz<D>(lrow0 + e * kRows);
+    lcol[e] = (uint32_t)(c < last16 ? c : last16) * 16;
   }
   const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_k;
   const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_v;
-  int blk0 = 0, key_lo = 0, key_hi = 0;    // of the segment: first block listed, keys loaded
-  auto div_bs = [&](int x) { return a.bs_shift >= 0 ? x >> a.bs_shift : x / bs; };
-  auto pool_row = [&](int step, int e) -> int64_t {
-    const int key = clampi(step * KT + lrow[e], key_lo, key_hi - 1);
-    const int lb = div_bs(key);
-    return (int64_t)s_row[lb - blk0] + (key - lb * bs);
+  // s_row lists the first pool row of each block, or, where the block size is no
+  // power of two, of each key
+  const int sh = a.bs_shift >= 0 ? a.bs_shift : 0, in_blk = (1 << sh) - 1;
+  int ent0 = 0, key_lo = 0, key_hi = 0;    // of the segment: first entry listed, keys loaded
+  auto pool_at = [&](int step, int e) -> int64_t {   // byte offset of this lane's load e
+    const int key = max(key_lo, min(key_hi - 1, step * KT + lrow0 + e * kRows));
+    return (int64_t)((uint64_t)(uint32_t)(s_row[(key >> sh) - ent0] + (key & in_blk)) * (uint32_t)rowb) + lcol[e];
   };
-  auto load = [&](int step, int b) {        // 2-byte pools
+  auto load = [&](int step, int buf) {   // 2-byte pools
 #pragma unroll
     for (int e = 0; e < NR; ++e) {
-      const int64_t off = pool_row(step, e) * rowb + lcol[e];
-      const uint32_t run = (uint32_t)(b * TB + (wave * NI + e) * 1024);
-      load_to_lds(lds_k + run, a.k_cache + off);
-      load_to_lds(lds_v + run, a.v_cache + off);
+      const int64_t at = pool_at(step, e);
+      const uint32_t run = (uint32_t)(buf * TB + (wave * NI + e) * 1024);
+      load_to_lds(lds_k + run, a.k_cache + at);
+      load_to_lds(lds_v + run, a.v_cache + at);
     }
   };
-  u32x4 rk[kF8 ? NR : 1], rv[kF8 ? NR : 1];
-  auto fetch = [&](int step) {              // FP8 pools: bytes into registers ...
+  struct Raw {
+    u32x4 w[kF8 ? NR : 1];
+  };
+  auto fetch = [&](int step, Raw& rk, Raw& rv) {   // FP8 pools: bytes into registers ...
+    if (kSome && tid >= KT * LROW) return;
 #pragma unroll
     for (int e = 0; e < NR; ++e) {
-      const int64_t off = pool_row(step, e) * rowb + lcol[e];
-      rk[kF8 ? e : 0] = *reinterpret_cast<const u32x4*>(a.k_cache + off);
-      rv[kF8 ? e : 0] = *reinterpret_cast<const u32x4*>(a.v_cache + off);
+      const int64_t at = pool_at(step, e);
+      rk.w[kF8 ? e : 0] = *reinterpret_cast<const u32x4*>(a.k_cache + at);
+      rv.w[kF8 ? e : 0] = *reinterpret_cast<const u32x4*>(a.v_cache + at);
     }
   };
-  auto stash = [&](int b) {                 // ... and converted into LDS
+  auto stash = [&](const Raw& rk, const Raw& rv, int buf) {   // ... and converted into LDS
+    if (kSome && tid >= KT * LROW) return;
 #pragma unroll
     for (int e = 0; e < NR; ++e) {
-      const int c = (tid + kThreads * e) % LROW * 2, sw = swz<D>(lrow[e]);
-      const int at = b * TB + lrow[e] * RB;
-      const u32x4 k = rk[kF8 ? e : 0], v = rv[kF8 ? e : 0];
+      const int c = tid % LROW * 2, row = lrow0 + e * kRows, sw = swz<D>(row);
+      const int at = buf * TB + row * RB;
+      const u32x4 k = rk.w[kF8 ? e : 0], v = rv.w[kF8 ? e : 0];
       *reinterpret_cast<u32x4*>(s_k + at + ((c ^ sw) << 4)) = e4m3x8_to<TT>(k.x, k.y);
       *reinterpret_cast<u32x4*>(s_k + at + (((c + 1) ^ sw) << 4)) = e4m3x8_to<TT>(k.z, k.w);
       *reinterpret_cast<u32x4*>(s_v + at + ((c ^ sw) << 4)) = e4m3x8_to<TT>(v.x, v.y);
@@ -289,104 +439,109 @@ void rows_kernel(Args a) {
   const int vrow = 4 * hf + ((lane & 15) >> 2);
   const int vofs = vrow * RB + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ swz<D>(vrow)) << 4) +
                    (lane & 1) * 8;
-  auto compute = [&](int step, int b) {
-    const int key0 = step * KT;
-    const bool some = (key0 < w_hi && key0 + KT > w_lo) || (key0 < w_pre && key0 + KT > w_first);
-    if (!some) return;     // no row of this wave sees a key here
-    f32x16 sacc[NS];       // S^T[key 32 n + 8 (i/4) + 4 hf + i%4][row c32]
+  // Exponent arguments are S * cs + off + nmref. Without a cap or slopes S is the
+  // product itself; with a plain cap S = 1 / (1 + e^2y), whose last step A - 2A S
+  // joins the exponent's FMA; else S is the score in log2 units.
+  constexpr bool kUnit = kBias || kCapped == kWideCap, kRecip = kCapped == kPlainCap && !kBias;
+  const float cs = kUnit ? 1.f : (kRecip ? -2.f * capA : c2);
+  const float off = kRecip ? capA : 0.f;
+  const float hidden = kRecip ? INFINITY : -INFINITY;   // S of a masked key
+  constexpr bool kBySum = std::is_same<TT, F16>::value;
+  constexpr int NPV = KB * DB;    // P.V operands of a step
+  constexpr f32x16 kZero = {0};
+
+  // Step i over the K and V tiles kt, vt
+  auto step = [&](int i, const char* kt, const char* vt) {
+    const int key0 = i * KT;
+    f32x16 s;   // S^T[key 8 (i/4) + 4 hf + i%4][row c32]
+    {
+      u32x4 ka[NC];
+      auto read = [&](int x) { ka[x] = *reinterpret_cast<const u32x4*>(kt + (kofs ^ (x << 5))); };
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+      for (int x = 0; x < kAhead; ++x) read(x);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sacc[n][i] = 0.f;
-#pragma unroll
-    for (int x = 0; x < NS * NC; ++x) {
-      const u32x4 ka = *reinterpret_cast<const u32x4*>(s_k + ((b * TB + kofs) ^ (x / NS << 5)) +
-                                                       x % NS * 32 * RB);
-      sacc[x % NS] = Mma<TT>::m32(ka, qb[x / NS], sacc[x % NS]);
+      for (int x = 0; x < NC; ++x) {
+        if (x + kAhead < NC) read(x + kAhead);
+        s = Mma<TT>::m32(ka[x], qb[x], x == 0 ? kZero : s);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    // scores in log2 units (without a cap or slopes: times c2 in the exponent)
-    if constexpr (kCap) {
-      if (__builtin_expect(a.cap_wide, 0)) {
+    if constexpr (kCapped == kPlainCap) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
+      for (int e = 0; e < 16; ++e) {
+        const float x = s[e];
+        const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * cin) + 1.f);
+        s[e] = kBias ? fmaf(-2.f * capA, r, capA) : r;
+      }
+    } else if constexpr (kCapped == kWideCap) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sacc[n][i] = cap_exact(sacc[n][i], cin, capA);
-      } else {
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sacc[n][i] = cap_plain(sacc[n][i], cin, capA);
+      for (int e = 0; e < 16; ++e) {
+        const float x = s[e];
+        s[e] = cap_exact(x, cin, capA);
       }
     }
     if constexpr (kBias) {
       const float dist0 = (float)(pos - key0 - 4 * hf);
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float dist = fabsf(dist0 - (float)(n * 32 + 8 * (i >> 2) + (i & 3)));
-          const float x = sacc[n][i];
-          sacc[n][i] = fmaf(-slope, dist, kCap ? x : x * c2);
-        }
+      for (int e = 0; e < 16; ++e) {
+        const float x = s[e], dist = fabsf(dist0 - (float)(8 * (e >> 2) + (e & 3)));
+        s[e] = fmaf(-slope, dist, kCap ? x : x * c2);
+      }
     }
-    const bool all = (key0 >= w_lo1 && key0 + KT <= w_hi0) || (key0 >= w_first1 && key0 + KT <= w_pre0);
-    if (!all) {
+    const bool whole = (key0 >= w_lo1 && key0 + KT <= w_hi0) || (key0 >= w_first1 && key0 + KT <= w_pre0);
+    if (!whole) {
       const int o = key0 + 4 * hf;
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = o + n * 32 + 8 * (i >> 2) + (i & 3);
-          const bool seen = (key >= see.lo && key < see.hi) || (key >= see.first && key < see.pre);
-          const float x = sacc[n][i];
-          sacc[n][i] = seen ? x : -INFINITY;
-        }
+      for (int e = 0; e < 16; ++e) {
+        const int key = o + 8 * (e >> 2) + (e & 3);
+        const bool seen = (key >= see.lo && key < see.hi) || (key >= see.first && key < see.pre);
+        const float x = s[e];
+        s[e] = seen ? x : hidden;
+      }
     }
-    constexpr bool kScaled = !kCap && !kBias;
-    const float cs = kScaled ? c2 : 1.f;
-    u32x4 pb[KB];   // P^T as B operands: slots e < 4 -> key 4 hf + e, e >= 4 -> 8 + 4 hf + e - 4
+    // P^T as B operands: slots e < 4 -> key 4 hf + e, e >= 4 -> 8 + 4 hf + e - 4
+    // (pairs of scalars up to the products: vectors here are put together in an
+    // else branch of the rare case below, and every accumulator is copied for it)
+    uint32_t pb[8];
     auto expo = [&]() {
+      const float o = off + nmref;
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float x = sacc[n][i], y = sacc[n][i + 1];
-          pb[n * 2 + (i >> 3)][(i & 7) >> 1] =
-              TT::pack2(__builtin_amdgcn_exp2f(kScaled ? fmaf(x, cs, nmref) : x + nmref),
-                        __builtin_amdgcn_exp2f(kScaled ? fmaf(y, cs, nmref) : y + nmref));
-        }
+      for (int e = 0; e < 16; e += 2) {
+        const float x = s[e], y = s[e + 1];
+        pb[e >> 1] = TT::pack2(__builtin_amdgcn_exp2f(kUnit ? x + o : fmaf(x, cs, o)),
+                                             __builtin_amdgcn_exp2f(kUnit ? y + o : fmaf(y, cs, o)));
+      }
     };
     auto sum_p = [&](float x) {
-      float ps[4] = {x, 0.f, 0.f, 0.f};
+      float y = 0.f;
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ps[i] = TT::dot2(pb[kb][i], TT::kOne2, ps[i]);
-      return (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      for (int e = 0; e < 8; e += 2) {
+        x = TT::dot2(pb[e], TT::kOne2, x);
+        y = TT::dot2(pb[e + 1], TT::kOne2, y);
+      }
+      return x + y;
     };
     expo();
-    constexpr bool kBySum = std::is_same<TT, F16>::value;
     float st = 0.f;
     bool past;
     if constexpr (kBySum) {
       st = sum_p(0.f);
       past = !(st < Bound<TT>::kPast);
     } else {
-      uint32_t o = 0;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        o = o | pb[kb][0] | pb[kb][1];
-        o = o | pb[kb][2] | pb[kb][3];
-      }
-      past = (o & 0x40004000u) != 0;
+      uint32_t o = pb[0] | pb[1] | pb[2];
+      o = o | pb[3] | pb[4];
+      o = o | pb[5] | pb[6];
+      past = ((o | pb[7]) & 0x40004000u) != 0;
     }
-    if (__ballot(past) != 0) {
+    if (__builtin_expect(__ballot(past) != 0, 0)) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[n][i]);
-      mx = half_max(mx) * cs;
+      for (int e = 0; e < 16; ++e) {
+        const float x = s[e];
+        mx = fmaxf(mx, kUnit ? x : fmaf(x, cs, off));
+      }
+      mx = half_max(mx);
       const bool nd = mx > mref + Bound<TT>::kMove;
       const float mnew = nd ? mx + Bound<TT>::kBias : mref;
       const float alpha = nd ? __builtin_amdgcn_exp2f(mref - mnew) : 1.f;   // 0 from -inf
@@ -398,57 +553,75 @@ void rows_kernel(Args a) {
       expo();
       if constexpr (kBySum) st = sum_p(0.f);
     }
+    u32x4 va[NPV];
+    auto read = [&](int x) {   // 16-key block x / DB, 32-dim block x % DB
+      const int at = vofs ^ (x % DB << 6);
+      const u32x2 lo = lds_read_tr(vt + at + x / DB * 16 * RB);
+      const u32x2 hi = lds_read_tr(vt + (at ^ swz8<D>()) + (x / DB * 16 + 8) * RB);
+      va[x] = u32x4{lo.x, lo.y, hi.x, hi.y};
+    };
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) read(x);
     if constexpr (kBySum) lsum += st;
     else lsum = sum_p(lsum);
-    const int vt = b * TB + vofs;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const int at = vt ^ (db << 6);
-        const u32x2 lo = lds_read_tr(s_v + at + kb * 16 * RB);
-        const u32x2 hi = lds_read_tr(s_v + (at ^ swz8<D>()) + (kb * 16 + 8) * RB);
-        oacc[db] = Mma<TT>::m32(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[kb], oacc[db]);
-      }
+    for (int x = 0; x < NPV; ++x) {
+      if (x + kAhead < NPV) read(x + kAhead);
+      oacc[x % DB] = Mma<TT>::m32(va[x], u32x4{pb[x / DB * 4], pb[x / DB * 4 + 1], pb[x / DB * 4 + 2],
+                                                 pb[x / DB * 4 + 3]}, oacc[x % DB]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   // ---- the part's steps, from the last back: near ones, then far ones, each in
-  // segments whose blocks fit the list
-  const int64_t list_steps = (int64_t)(kListBlocks - 2) * bs / KT;
-  const int seg = list_steps < 1 ? 1 : (list_steps > 1 << 20 ? 1 << 20 : (int)list_steps);
-  for (int range = 1; range >= 0; --range) {
-    // steps of this range in the part: [r0, r1)
-    const int r0 = range ? ns0 + max(st0 - nfar, 0) : fs0 + min(st0, nfar);
-    const int r1 = range ? ns0 + max(st1 - nfar, 0) : fs0 + min(st1, nfar);
-    const int k0 = range ? nk0 : fk0, k1 = range ? nk1 : fk1;
-    for (int e1 = r1; e1 > r0; e1 -= seg) {
-      const int e0 = e1 - seg > r0 ? e1 - seg : r0;
-      key_lo = max(k0, e0 * KT);
-      key_hi = min(k1, e1 * KT);
-      __syncthreads();       // the last segment's reads are done
-      blk0 = div_bs(key_lo);
-      const int nblk = div_bs(key_hi - 1) + 1 - blk0;
-      for (int e = tid; e < nblk; e += kThreads) {
-        const int bid = clampi(a.block_tables[(int64_t)it.s * a.max_bps + blk0 + e], 0, a.num_blocks - 1);
-        s_row[e] = (bid * a.num_kv_heads + kh) * bs;
-      }
-      wait_all_and_barrier();
+  // segments whose blocks fit the list. Count n up from a segment's last step; tile
+  // n + kBufs - 1 starts loading in step n, into the buffer that step n - 1 read.
+  const int64_t list_steps = ((int64_t)(kListEntries - 2) << sh) / KT;
+  const int seg = list_steps > 1 << 20 ? 1 << 20 : (int)list_steps;
+  Raw rk, rv;
+  for (int c = st1 - 1; c >= st0;) {
+    const bool near = c >= nfar;
+    const int c0 = max(max(st0, near ? nfar : 0), c - seg + 1);
+    const int N = c - c0 + 1, top = near ? ns0 + (c - nfar) : fs0 + c;
+    c = c0 - 1;
+    key_lo = max(near ? nk0 : fk0, (top + 1 - N) * KT);
+    key_hi = min(near ? nk1 : fk1, (top + 1) * KT);
+    __syncthreads();       // the last segment's reads are done
+    ent0 = key_lo >> sh;
+    const int nent = ((key_hi - 1) >> sh) + 1 - ent0;
+    for (int e = tid; e < nent; e += kThreads) {
+      const int key = (ent0 + e) << sh, lb = a.bs_shift >= 0 ? ent0 + e : key / bs;
+      const int bid = clampi(a.block_tables[(int64_t)it.s * a.max_bps + lb], 0, a.num_blocks - 1);
+      s_row[e] = (bid * a.num_kv_heads + kh) * bs + (key - lb * bs);
+    }
+    // none of the compiler's own loads stays in flight: its waits inside the loop
+    // would cover the tile loads too
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    __syncthreads();
+    if constexpr (kF8) {
+      fetch(top, rk, rv);
+      stash(rk, rv, 0);
+    } else {
+      load(top, 0);
+      if (kBufs > 2 && N > 1) load(top - 1, 1);
+    }
+    int buf = 0;
+    for (int n = 0; n < N; ++n) {
+      const int next = buf == kBufs - 1 ? 0 : buf + 1;
       if constexpr (kF8) {
-        fetch(e1 - 1);
-        stash(0);
+        wait_and_barrier<63>();
+        if (n + 1 < N) fetch(top - n - 1, rk, rv);
       } else {
-        load(e1 - 1, 0);
+        if (kBufs > 2 && n + 1 < N) wait_and_barrier<2 * NR>();   // tile n + 1 may be in flight
+        else wait_and_barrier<0>();
+        if (n + kBufs - 1 < N) load(top - n - (kBufs - 1), buf == 0 ? kBufs - 1 : buf - 1);
       }
-      for (int i = e1 - 1, b = 0; i >= e0; --i, b ^= 1) {
-        wait_all_and_barrier();    // tile i is there, and all waves have left the other buffer
-        if (i > e0) {
-          if constexpr (kF8) fetch(i - 1); else load(i - 1, b ^ 1);
-        }
-        compute(i, b);
-        if constexpr (kF8) {
-          if (i > e0) stash(b ^ 1);
-        }
+      step(top - n, s_k + buf * TB, s_v + buf * TB);
+      if constexpr (kF8) {
+        if (n + 1 < N) stash(rk, rv, next);
       }
+      buf = next;
     }
   }
 
@@ -458,82 +631,72 @@ void rows_kernel(Args a) {
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) chk = fmaf(oacc[db][i], 0.f, chk);
-  const bool bad = !(chk < INFINITY);          // an infinity or NaN among the row's sums
-  const uint32_t bad32 = (uint32_t)__ballot(bad) | (uint32_t)(__ballot(bad) >> 32);
-  const bool mine_bad = (bad32 >> c32) & 1;
+    for (int i = 0; i < 16; ++i) {
+      const float x = oacc[db][i];
+      chk = fmaf(x, 0.f, chk);
+    }
+  const uint64_t bad = __ballot(!(chk < INFINITY));   // an infinity or NaN among the row's sums
+  const uint32_t bad_rows = (uint32_t)bad | (uint32_t)(bad >> 32);
   const float oscale = kF8 ? a.v_scale[kh] : 1.f;
-  const int64_t slot0 = ((tile * a.num_kv_heads + kh) * a.tile_splits + part) * kTileRows + wave * 32;
-  if (row_ok && !mine_bad) {
-    if (!merged) {
-      const float inv = ltot > 0.f ? oscale / ltot : 0.f;
+  const int64_t slot0 = (int64_t)blockIdx.x * TR + wave * 32;
+  if (row_ok && !((bad_rows >> c32) & 1)) {
+    const float inv = ltot > 0.f ? oscale / ltot : 0.f;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = db * 32 + i * 8 + hf * 4;
-          if (e < d)
-            *reinterpret_cast<u32x2*>(op + e) =
-                u32x2{TT::pack2(oacc[db][4 * i] * inv, oacc[db][4 * i + 1] * inv),
-                      TT::pack2(oacc[db][4 * i + 2] * inv, oacc[db][4 * i + 3] * inv)};
-        }
-    } else {
-      float* po = a.tile_o + (slot0 + c32) * d;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = db * 32 + i * 8 + hf * 4;
-          if (e < d)
-            *reinterpret_cast<f32x4*>(po + e) = f32x4{oacc[db][4 * i], oacc[db][4 * i + 1],
-                                                      oacc[db][4 * i + 2], oacc[db][4 * i + 3]};
-        }
-      if (hf == 0) {
-        a.tile_ml[(slot0 + c32) * 2] = mref;
-        a.tile_ml[(slot0 + c32) * 2 + 1] = ltot;
+      for (int i = 0; i < 4; ++i) {
+        const int e = db * 32 + i * 8 + hf * 4;
+        if (e >= d) continue;
+        const f32x4 v = f32x4{oacc[db][4 * i], oacc[db][4 * i + 1], oacc[db][4 * i + 2], oacc[db][4 * i + 3]};
+        if (merged)
+          *reinterpret_cast<f32x4*>(a.tile_o + (slot0 + c32) * d + e) = v;
+        else
+          *reinterpret_cast<u32x2*>(op + e) =
+              u32x2{TT::pack2(v.x * inv, v.y * inv), TT::pack2(v.z * inv, v.w * inv)};
       }
+    if (merged && hf == 0) {
+      a.tile_ml[(slot0 + c32) * 2] = mref;
+      a.tile_ml[(slot0 + c32) * 2 + 1] = ltot;
     }
   }
-  if (__builtin_expect(bad32 == 0, 1)) return;
+  if (__builtin_expect(bad_rows == 0, 1)) return;
 
   // ---- redo of rows whose sums are not finite: one key after another, over the
   // keys that the row sees in this part; lane l holds dims 4l .. 4l + 3
-  for (int r = 0; r < 32; ++r) {
-    if (!((bad32 >> r) & 1) || f0 + r >= it.rows) continue;
-    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, r); };
+  for (int w = 0; w < 32; ++w) {
+    if (!((bad_rows >> w) & 1) || f0 + w >= frows) continue;
+    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, w); };
     const int rlo = of(see.lo), rhi = of(see.hi), rfirst = of(see.first), rpre = of(see.pre);
     const int rpos = of(pos), rtok = of(qrow), rh = of(h);
     const float rslope = kBias ? a.slopes[rh] * kLog2e : 0.f;
-    const int e0 = lane * 4;
-    const bool on = e0 < d;
+    const int d0 = lane * 4;
+    const bool on = d0 < d;
+    auto widen = [](u32x2 x, float (&f)[4]) {
+      f[0] = TT::lo(x.x), f[1] = TT::hi(x.x), f[2] = TT::lo(x.y), f[3] = TT::hi(x.y);
+    };
     float qv[4] = {0, 0, 0, 0}, o[4] = {0, 0, 0, 0};
-    if (on) {
-      const u32x2 w = *reinterpret_cast<const u32x2*>(a.q + (int64_t)rtok * a.q_stride_token +
-                                                      (int64_t)rh * a.q_stride_head + e0);
-      qv[0] = TT::lo(w.x), qv[1] = TT::hi(w.x), qv[2] = TT::lo(w.y), qv[3] = TT::hi(w.y);
-    }
+    if (on)
+      widen(*reinterpret_cast<const u32x2*>(a.q + (int64_t)rtok * a.q_stride_token +
+                                            (int64_t)rh * a.q_stride_head + d0), qv);
     float m = -INFINITY, l = 0.f;
     for (int i = st0; i < st1; ++i) {
       const int step = i < nfar ? fs0 + i : ns0 + (i - nfar);
       for (int key = step * KT; key < step * KT + KT; ++key) {
         if (!((key >= rlo && key < rhi) || (key >= rfirst && key < rpre))) continue;
-        const int lb = div_bs(key);
+        const int lb = a.bs_shift >= 0 ? key >> a.bs_shift : key / bs;
         const int bid = clampi(a.block_tables[(int64_t)it.s * a.max_bps + lb], 0, a.num_blocks - 1);
-        const int64_t off = ((int64_t)(bid * a.num_kv_heads + kh) * bs + (key - lb * bs)) * rowb + e0 * EB;
+        const int64_t at = ((int64_t)(bid * a.num_kv_heads + kh) * bs + (key - lb * bs)) * rowb + d0 * EB;
         float kv[4] = {0, 0, 0, 0}, vv[4] = {0, 0, 0, 0};
         if (on) {
-          u32x2 kw, vw;
           if constexpr (kF8) {
-            const uint32_t kb = *reinterpret_cast<const uint32_t*>(a.k_cache + off);
-            const uint32_t vb = *reinterpret_cast<const uint32_t*>(a.v_cache + off);
-            kw = u32x2{e4m3x2_to<TT, false>(kb), e4m3x2_to<TT, true>(kb)};
-            vw = u32x2{e4m3x2_to<TT, false>(vb), e4m3x2_to<TT, true>(vb)};
+            const uint32_t kw = *reinterpret_cast<const uint32_t*>(a.k_cache + at);
+            const uint32_t vw = *reinterpret_cast<const uint32_t*>(a.v_cache + at);
+            widen(u32x2{e4m3x2_to<TT, false>(kw), e4m3x2_to<TT, true>(kw)}, kv);
+            widen(u32x2{e4m3x2_to<TT, false>(vw), e4m3x2_to<TT, true>(vw)}, vv);
           } else {
-            kw = *reinterpret_cast<const u32x2*>(a.k_cache + off);
-            vw = *reinterpret_cast<const u32x2*>(a.v_cache + off);
+            widen(*reinterpret_cast<const u32x2*>(a.k_cache + at), kv);
+            widen(*reinterpret_cast<const u32x2*>(a.v_cache + at), vv);
           }
-          kv[0] = TT::lo(kw.x), kv[1] = TT::hi(kw.x), kv[2] = TT::lo(kw.y), kv[3] = TT::hi(kw.y);
-          vv[0] = TT::lo(vw.x), vv[1] = TT::hi(vw.x), vv[2] = TT::lo(vw.y), vv[3] = TT::hi(vw.y);
         }
         float t = fmaf(qv[0], kv[0], qv[1] * kv[1]) + fmaf(qv[2], kv[2], qv[3] * kv[3]);
         t = wave_sum_f(t);
@@ -552,13 +715,14 @@ void rows_kernel(Args a) {
       const float inv = l > 0.f || l != l ? oscale / l : 0.f;
       if (on)
         *reinterpret_cast<u32x2*>(a.out + (int64_t)rtok * a.out_stride_token +
-                                  (int64_t)rh * a.out_stride_head + e0) =
+                                  (int64_t)rh * a.out_stride_head + d0) =
             u32x2{TT::pack2(o[0] * inv, o[1] * inv), TT::pack2(o[2] * inv, o[3] * inv)};
     } else {
-      if (on) *reinterpret_cast<f32x4*>(a.tile_o + (slot0 + r) * d + e0) = f32x4{o[0], o[1], o[2], o[3]};
+      const int64_t slot = slot0 + w;
+      if (on) *reinterpret_cast<f32x4*>(a.tile_o + slot * d + d0) = f32x4{o[0], o[1], o[2], o[3]};
       if (lane == 0) {
-        a.tile_ml[(slot0 + r) * 2] = m;
-        a.tile_ml[(slot0 + r) * 2 + 1] = l;
+        a.tile_ml[slot * 2] = m;
+        a.tile_ml[slot * 2 + 1] = l;
       }
     }
   }
@@ -566,13 +730,18 @@ void rows_kernel(Args a) {
 
 template <class TT, int D, bool kF8>
 void launch_rows_f(const Args& a, hipStream_t st) {
-  const int64_t tiles = a.cu_seqlens_q ? (int64_t)a.num_seqs * a.tiles_max : a.tiles;
-  const dim3 g((unsigned)(tiles * a.num_kv_heads * a.tile_splits)), b(kThreads);
-  const bool cap = a.cap_log2 > 0.f, bias = a.slopes != nullptr;
-  if (cap && bias) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, true, true>), g, b, 0, st, a);
-  else if (cap) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, true, false>), g, b, 0, st, a);
-  else if (bias) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, false, true>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((rows_kernel<TT, D, kF8, false, false>), g, b, 0, st, a);
+  const dim3 g((unsigned)(a.items * a.num_kv_heads)), b(kThreads);
+  const bool bias = a.slopes != nullptr;
+  if (a.cap_log2 <= 0.f) {
+    if (bias) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kNoCap, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kNoCap, false>), g, b, 0, st, a);
+  } else if (a.cap_wide) {
+    if (bias) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kWideCap, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kWideCap, false>), g, b, 0, st, a);
+  } else {
+    if (bias) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kPlainCap, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kPlainCap, false>), g, b, 0, st, a);
+  }
 }
 
 template <int D>

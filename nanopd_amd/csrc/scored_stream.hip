@@ -264,7 +264,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
   const int kh = h / a.group, hh = h - kh * a.group, d = a.head_dim;
   int nt = 0, nu = 0;        // partials of tiles and of stream units
   int64_t tslot = 0, uslot = 0;
-  const int tstep = kTileRows;   // a tile's parts are kTileRows slots apart
+  const int64_t tstep = (int64_t)a.num_kv_heads * kTileRows;   // slots between a tile's parts
   if (a.cu_seqlens_q) {
     // the sequence of the token: the last that starts at or before it (binary search)
     int lo = 0, hi = a.num_seqs - 1;
@@ -278,9 +278,10 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
     const int f = (tok - q0) * a.group + hh;
     if (f / kTileRows >= a.tiles_max) return;
     const int64_t tile = (int64_t)q0 * a.group / kTileRows + lo + f / kTileRows;
-    nt = a.tile_parts[tile * a.num_kv_heads + kh];
+    const int32_t* ti = a.tile_items + 2 * (tile * a.num_kv_heads + kh);
+    nt = ti[1];
     if (nt <= 1) return;     // written by the rows kernel itself
-    tslot = (tile * a.num_kv_heads + kh) * a.tile_splits * kTileRows + f % kTileRows;
+    tslot = ((int64_t)ti[0] * a.num_kv_heads + kh) * kTileRows + f % kTileRows;
   } else {
     int pos, a0, na, b0, nb;
     unit_keys(a, tok, lane, pos, a0, na, b0, nb);
@@ -288,21 +289,25 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
     if (!a.cu_groups && nu <= 1) return;   // written by the stream kernel itself
     uslot = ((int64_t)tok * a.num_heads + h) * a.unit_splits;
     Group g;
-    if (a.cu_groups && find_group<true>(a, tok, lane, g)) {
+    if (a.cu_groups && find_group<true>(a, tok, lane, g) && g.shared > 0) {
       const int64_t f = (int64_t)(tok - g.seq0) * a.group + hh;
       const int64_t tile = g.tile0 + f / kTileRows;
       if (tile < a.tiles) {
-        nt = a.tile_parts[tile * a.num_kv_heads + kh];
-        tslot = (tile * a.num_kv_heads + kh) * a.tile_splits * kTileRows + f % kTileRows;
+        const int32_t* ti = a.tile_items + 2 * (tile * a.num_kv_heads + kh);
+        nt = ti[1];
+        tslot = ((int64_t)ti[0] * a.num_kv_heads + kh) * kTileRows + f % kTileRows;
       }
     }
   }
+  // (lists that do not ascend may leave an entry unwritten: stay in the buffer)
+  const int64_t room = (int64_t)a.items * a.num_kv_heads * kTileRows;
+  if (tslot < 0 || nt < 0 || tslot + nt * tstep > room + tstep - kTileRows) nt = 0;
   const int n = nt + nu;
   auto ml = [&](int i) {
-    return i < nt ? a.tile_ml + (tslot + (int64_t)i * tstep) * 2 : a.unit_ml + (uslot + i - nt) * 2;
+    return i < nt ? a.tile_ml + (tslot + i * tstep) * 2 : a.unit_ml + (uslot + i - nt) * 2;
   };
   auto ov = [&](int i) {
-    return i < nt ? a.tile_o + (tslot + (int64_t)i * tstep) * d : a.unit_o + (uslot + i - nt) * d;
+    return i < nt ? a.tile_o + (tslot + i * tstep) * d : a.unit_o + (uslot + i - nt) * d;
   };
   float M = -INFINITY;
   for (int i = lane; i < n; i += 64) M = fmaxf(M, ml(i)[0]);
@@ -313,6 +318,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
   if (M > -INFINITY) {
     for (int i = lane / LPR; i < n; i += SG) {
       const float* p = ml(i);
+      if (p[0] == -INFINITY) continue;   // a part without a key
       const float w = __builtin_amdgcn_exp2f(p[0] - M);
       L = fmaf(p[1], w, L);
       if (c < d) {
@@ -381,17 +387,10 @@ int64_t unit_splits_of(int64_t units, int64_t max_keys) {
   return w < 1 ? 1 : w;
 }
 
-// Most parts of a tile of the rows kernel: enough for two workgroups per compute
-// unit (one at head dims above 128), none shorter than kMinTileSteps steps.
-constexpr int64_t kMinTileSteps = 4, kMaxTileSplits = 64;
-int64_t tile_splits_of(int64_t tiles, int64_t head_dim, int64_t max_keys, bool shared) {
-  const int64_t room = (head_dim > 128 ? 1 : 2) * (int64_t)device_cus();
-  const int64_t steps = max_keys / kStepKeys + 2;
-  int64_t p = room / (tiles < 1 ? 1 : tiles);
-  p = p < steps / kMinTileSteps ? p : steps / kMinTileSteps;
-  p = p < kMaxTileSplits ? p : kMaxTileSplits;
-  (void)shared;
-  return p < 1 ? 1 : p;
+// Workgroups of the rows kernel that run at once per kv head.
+int64_t rows_room(int64_t head_dim, int64_t num_kv_heads) {
+  const int64_t n = rows_per_cu(head_dim) * (int64_t)device_cus() / num_kv_heads;
+  return n < 1 ? 1 : n;
 }
 
 int64_t pad256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -400,10 +399,11 @@ int64_t pad256(int64_t x) { return (x + 255) / 256 * 256; }
 // ops leave alone, so that one buffer serves every attention op), then the
 // tiles' partials and part counts, then the units'.
 struct Plan {
-  int64_t tiles = 0, tiles_max = 0, tile_splits = 1, unit_splits = 1;
+  int64_t tiles = 0, tiles_max = 0, items = 0, room = 1, unit_splits = 1;
+  bool list = false;
   int64_t tile_slots = 0, unit_slots = 0, head_dim = 0, kv_heads = 0;
-  int64_t parts_at() const { return kCounterBytes; }
-  int64_t tile_o_at() const { return parts_at() + (tile_slots ? pad256(tiles * kv_heads * 4) : 0); }
+  int64_t tile_items_at() const { return kCounterBytes; }
+  int64_t tile_o_at() const { return tile_items_at() + (tile_slots ? pad256(tiles * kv_heads * 8) : 0); }
   int64_t tile_ml_at() const { return tile_o_at() + pad256(tile_slots * head_dim * 4); }
   int64_t unit_o_at() const { return tile_ml_at() + pad256(tile_slots * 8); }
   int64_t unit_ml_at() const { return unit_o_at() + pad256(unit_slots * head_dim * 4); }
@@ -429,8 +429,13 @@ Plan shared_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int6
   Plan p = decode_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_keys);
   p.unit_slots = num_seqs * num_heads * p.unit_splits;   // always merged
   p.tiles = num_seqs * (num_heads / num_kv_heads) / kTileRows + num_groups;
-  p.tile_splits = tile_splits_of(p.tiles * num_kv_heads, head_dim, max_shared, true);
-  p.tile_slots = p.tiles * num_kv_heads * p.tile_splits * kTileRows;
+  p.list = true;
+  p.room = rows_room(head_dim, num_kv_heads);
+  // parts of target steps: at most room + one round-up per tile, nor more than
+  // the shared keys' steps
+  const int64_t most = p.tiles * (max_shared / kStepKeys + 1);
+  p.items = p.room + p.tiles < most ? p.room + p.tiles : most;
+  p.tile_slots = p.items * num_kv_heads * kTileRows;
   return p;
 }
 Plan chunk_plan(int64_t num_seqs, int64_t total_q, int64_t num_heads, int64_t num_kv_heads,
@@ -441,9 +446,16 @@ Plan chunk_plan(int64_t num_seqs, int64_t total_q, int64_t num_heads, int64_t nu
   p.kv_heads = num_kv_heads;
   p.tiles = total_q * g / kTileRows + num_seqs;
   p.tiles_max = (max_q_len * g + kTileRows - 1) / kTileRows;
-  const int64_t most = num_seqs * p.tiles_max;
-  p.tile_splits = tile_splits_of((p.tiles < most ? p.tiles : most) * num_kv_heads, head_dim, max_keys, false);
-  p.tile_slots = p.tile_splits > 1 ? p.tiles * num_kv_heads * p.tile_splits * kTileRows : 0;
+  p.room = rows_room(head_dim, num_kv_heads);
+  p.items = num_seqs * p.tiles_max;
+  const int64_t most = p.tiles < p.items ? p.tiles : p.items;
+  // cut into parts unless whole tiles fill the chip three times over, or hold so
+  // few keys that none would be cut
+  p.list = p.items <= kListTiles && most < 3 * p.room && max_keys > 8 * kStepKeys;
+  if (p.list) {
+    p.items = p.room + most;
+    p.tile_slots = p.items * num_kv_heads * kTileRows;
+  }
   return p;
 }
 
@@ -533,7 +545,7 @@ Args make_args(const Call& c, const Plan& p, void* workspace) {
   a.v_scale = c.v_scale;
   char* ws = static_cast<char*>(workspace);
   if (p.tile_slots) {
-    a.tile_parts = reinterpret_cast<int32_t*>(ws + p.parts_at());
+    a.tile_items = reinterpret_cast<int32_t*>(ws + p.tile_items_at());
     a.tile_o = reinterpret_cast<float*>(ws + p.tile_o_at());
     a.tile_ml = reinterpret_cast<float*>(ws + p.tile_ml_at());
   }
@@ -553,7 +565,9 @@ Args make_args(const Call& c, const Plan& p, void* workspace) {
   a.max_bps = (int)c.max_bps;
   a.tiles = (int)p.tiles;
   a.tiles_max = (int)p.tiles_max;
-  a.tile_splits = (int)p.tile_splits;
+  a.items = (int)p.items;
+  a.room = (int)p.room;
+  a.list = p.list;
   a.unit_splits = (int)p.unit_splits;
   a.subs = (int)subs_of(a.group);
   a.sub_heads = (a.group + a.subs - 1) / a.subs;
@@ -660,16 +674,18 @@ extern "C" int npd_paged_attention_shared(
                 (long long)num_groups, (long long)max_shared_len);
   if (num_seqs == 0) return NPD_OK;
   if (!cu_groups || !shared_lens) return fail(NPD_E_INVALID, "%s: null pointer", c.name);
-  const Plan p = shared_plan(num_seqs, num_heads, num_kv_heads, head_dim,
-                             block_size * max_blocks_per_seq, num_groups, max_shared_len);
+  const int64_t max_keys = block_size * max_blocks_per_seq;
+  const Plan p = shared_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_keys, num_groups,
+                             max_shared_len);
   rc = check_workspace(c, p, workspace, workspace_bytes);
   if (rc != NPD_OK) return rc;
   Args a = make_args(c, p, workspace);
   a.cu_groups = cu_groups;
   a.shared_lens = shared_lens;
   a.num_groups = (int)num_groups;
+  a.max_shared = (int)(max_shared_len < max_keys ? max_shared_len : max_keys);
   if (!grid_ok(num_seqs * num_kv_heads * a.subs * p.unit_splits) ||
-      !grid_ok(p.tiles * num_kv_heads * p.tile_splits))
+      !grid_ok(p.items * num_kv_heads))
     return fail(NPD_E_INVALID, "%s: too many work items", c.name);
   hipStream_t st = as_stream(stream);
   launch_rows_any(a, dtype, st);
@@ -723,7 +739,7 @@ extern "C" int npd_paged_prefill_scored(
   a.cu_seqlens_q = cu_seqlens_q;
   a.first_keys = first_keys;
   a.prefix_lens = prefix_lens;
-  if (!grid_ok(num_seqs * p.tiles_max * num_kv_heads * p.tile_splits))
+  if (!grid_ok(p.items * num_kv_heads))
     return fail(NPD_E_INVALID, "%s: too many work items", c.name);
   hipStream_t st = as_stream(stream);
   launch_rows_any(a, dtype, st);

@@ -895,7 +895,7 @@ def paged_attention_shared(out: torch.Tensor, query: torch.Tensor, key_cache: to
     shared_lens[g] keys (int32 [num_groups]). seq_lens and block_tables are whole,
     as without groups. A sequence outside every group shares nothing; one shorter
     than its group's shared keys sees its own. ``max_shared_len``: a host-side
-    bound on shared_lens (it sets how many workgroups share the reading).
+    bound on shared_lens (shared keys past it are read per sequence).
     ``workspace``: at least :func:`shared_workspace_bytes` bytes.
     """
     s = query.size(0) if isinstance(query, torch.Tensor) and query.dim() == 3 else 0
