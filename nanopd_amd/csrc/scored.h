@@ -34,7 +34,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoRef = 3.402823466e38f;   // exponent offset of a row without a reference
 constexpr int kTileRows = 128;              // rows of a workgroup of the rows kernel
 // ... and how many of them run at once on a compute unit at (padded) head dim d
-__host__ __device__ constexpr int rows_per_cu(int64_t d) { return d > 128 ? 1 : d > 64 ? 2 : 3; }
+__host__ __device__ constexpr int rows_per_cu(int64_t d) { return d > 128 ? 1 : d > 64 ? 3 : 4; }
 constexpr int kStepKeys = 32;               // keys per step of the rows kernel
 constexpr int kListTiles = 512;             // most tiles per kv head that are cut into parts
 constexpr int kUnitHeads = 16;              // most heads of a stream unit (MFMA columns)
@@ -101,7 +101,7 @@ __device__ __forceinline__ float cap_exact(float x, float cin, float A) {
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
 // The keys a row sees: [lo, hi) and [first, pre), hi <= context.
-struct Keys {
+struct alignas(16) Keys {
   int first, lo, hi, pre;
 };
 __device__ __forceinline__ Keys row_keys(int pos, int ctx, int first, int pre, int window) {

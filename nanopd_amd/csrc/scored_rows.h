@@ -35,8 +35,7 @@ namespace npd {
 namespace scored {
 
 constexpr int kThreads = 256;
-constexpr int kListEntries = 1024;   // pool blocks listed in LDS at a time (4 KB)
-constexpr int kAhead = 4;            // LDS operand reads ahead of their MFMA
+constexpr int kListEntries = 512;    // pool blocks listed in LDS at a time
 constexpr int kMinPartSteps = 8;     // shortest part of a tile
 constexpr int kListSlots = kListTiles / 64;
 
@@ -242,6 +241,7 @@ void rows_kernel(Args a) {
   constexpr int KT = kStepKeys;
   constexpr int TR = kTileRows;
   constexpr int kBufs = D > 128 ? 2 : 3;    // K and V tiles in LDS
+  constexpr int kAhead = D > 128 ? 4 : 2;   // LDS operand reads ahead of their MFMA
   constexpr int RB = 2 * D;                 // bytes of a tile row
   constexpr int TB = KT * RB;               // bytes of a tile
   constexpr int NI = TB / 4096;             // 1 KB loads per wave and tile
@@ -253,6 +253,7 @@ void rows_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) char s_v[kBufs * TB];
   __shared__ int s_row[kListEntries];
   __shared__ int s_red[4][4];
+  __shared__ Keys s_see[TR];   // keys of the rows (read where a step masks)
   __shared__ Item s_item;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -290,25 +291,36 @@ void rows_kernel(Args a) {
 
   // ---- this lane's row (past the last: a copy of it, not stored)
   const int f0 = it.t * TR + wave * 32;
-  const bool row_ok = f0 + c32 < frows;
-  const int f = row_ok ? f0 + c32 : frows - 1;
-  const int tok = f / G;
-  const int h = kh * G + (f - tok * G);
-  const int qrow = it.row0 + tok;
+  struct Row {
+    bool ok;
+    int tok, h, q;     // token of the chunk or sequence of the group, head, row of q / out
+    __device__ int64_t strides(int64_t token, int64_t head) const { return q * token + h * head; }
+  };
+  auto row_of = [&](int c) {
+    Row r;
+    r.ok = f0 + c < frows;
+    const int f = r.ok ? f0 + c : frows - 1;
+    r.tok = f / G;
+    r.h = kh * G + (f - r.tok * G);
+    r.q = it.row0 + r.tok;
+    return r;
+  };
+  const Row row = row_of(c32);
   int pos, ctx;
   if (a.cu_seqlens_q) {
     ctx = it.limit;
-    pos = ctx - it.tokens + tok;
+    pos = ctx - it.tokens + row.tok;
   } else {
-    ctx = clampi(a.seq_lens[qrow], 0, cap_keys);
+    ctx = clampi(a.seq_lens[row.q], 0, cap_keys);
     pos = ctx - 1;
   }
-  Keys see = row_keys(pos, ctx, a.first_keys ? a.first_keys[qrow] : 0,
+  Keys see = row_keys(pos, ctx, a.first_keys ? a.first_keys[row.q] : 0,
                       a.prefix_lens ? a.prefix_lens[it.s] : 0, a.window);
   see.hi = min(see.hi, it.limit);
   see.pre = min(see.pre, it.limit);
   if (see.lo >= see.hi) see.lo = see.hi = 0;          // empty ranges are [0, 0)
   if (see.first >= see.pre) see.first = see.pre = 0;
+  if (hf == 0) s_see[wave * 32 + c32] = see;
 
   // ---- ranges: near [lo, hi), far [first, pre); of the wave (none where it has no
   // row to store) and of the workgroup the keys that some row sees, and of the wave
@@ -354,10 +366,9 @@ void rows_kernel(Args a) {
   const int st0 = it.part * base + min(it.part, rem), st1 = st0 + base + (it.part < rem ? 1 : 0);
 
   // ---- queries as B operands: qb[c] = Q[row][16c + 8 hf ..], zeros past the row
-  uint16_t* op = a.out + (int64_t)qrow * a.out_stride_token + (int64_t)h * a.out_stride_head;
   u32x4 qb[NC];
   {
-    const uint16_t* qp = a.q + (int64_t)qrow * a.q_stride_token + (int64_t)h * a.q_stride_head;
+    const uint16_t* qp = a.q + row.strides(a.q_stride_token, a.q_stride_head);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       qb[c] = c * 16 + hf * 8 < d ? *reinterpret_cast<const u32x4*>(qp + c * 16 + hf * 8)
@@ -365,7 +376,7 @@ void rows_kernel(Args a) {
   }
   const float kscale = kF8 ? a.k_scale[kh] : 1.f;
   const float c2 = a.scale_log2 * kscale, cin = a.cap_in * kscale, capA = a.cap_log2;
-  const float slope = kBias ? a.slopes[h] * kLog2e : 0.f;
+  const float slope = kBias ? a.slopes[row.h] * kLog2e : 0.f;
 
   // ---- tile loads. Chunks past the row's end repeat its last one (zero queries
   // meet them in S, and their output dims are not stored).
@@ -386,17 +397,37 @@ void rows_kernel(Args a) {
   const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_k;
   const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_v;
   // s_row lists the first pool row of each block, or, where the block size is no
-  // power of two, of each key
+  // power of two, of each key. A step that lies within the keys to load takes its
+  // rows by a list entry and an offset in the block that are a part of the lane's
+  // and a part of the step's; the others clamp key by key.
   const int sh = a.bs_shift >= 0 ? a.bs_shift : 0, in_blk = (1 << sh) - 1;
   int ent0 = 0, key_lo = 0, key_hi = 0;    // of the segment: first entry listed, keys loaded
-  auto pool_at = [&](int step, int e) -> int64_t {   // byte offset of this lane's load e
-    const int key = max(key_lo, min(key_hi - 1, step * KT + lrow0 + e * kRows));
-    return (int64_t)((uint64_t)(uint32_t)(s_row[(key >> sh) - ent0] + (key & in_blk)) * (uint32_t)rowb) + lcol[e];
+  // Of the tile loaded next: pool rows less the offsets off_blk + row_o (added where
+  // they are used, so that the wait for the list falls there)
+  int rows[NR], row_o = 0;
+  auto off_blk = [&](int e) { return (lrow0 + e * kRows) & in_blk; };
+  auto find_rows = [&](int step) {
+    const int k0 = step * KT;
+    row_o = k0 & in_blk;   // (0 for blocks up to KT)
+    if (k0 >= key_lo && k0 + KT <= key_hi) {
+      const int ent = (k0 >> sh) - ent0;
+#pragma unroll
+      for (int e = 0; e < NR; ++e) rows[e] = s_row[ent + ((lrow0 + e * kRows) >> sh)];
+    } else {
+#pragma unroll
+      for (int e = 0; e < NR; ++e) {
+        const int key = max(key_lo, min(key_hi - 1, k0 + lrow0 + e * kRows));
+        rows[e] = s_row[(key >> sh) - ent0] + (key & in_blk) - off_blk(e) - row_o;
+      }
+    }
   };
-  auto load = [&](int step, int buf) {   // 2-byte pools
+  auto byte_at = [&](int e) {   // of this lane's load e
+    return (int64_t)((uint64_t)(uint32_t)(rows[e] + off_blk(e) + row_o) * (uint32_t)rowb) + lcol[e];
+  };
+  auto load = [&](int buf) {   // 2-byte pools: the tile of `rows`
 #pragma unroll
     for (int e = 0; e < NR; ++e) {
-      const int64_t at = pool_at(step, e);
+      const int64_t at = byte_at(e);
       const uint32_t run = (uint32_t)(buf * TB + (wave * NI + e) * 1024);
       load_to_lds(lds_k + run, a.k_cache + at);
       load_to_lds(lds_v + run, a.v_cache + at);
@@ -405,11 +436,11 @@ void rows_kernel(Args a) {
   struct Raw {
     u32x4 w[kF8 ? NR : 1];
   };
-  auto fetch = [&](int step, Raw& rk, Raw& rv) {   // FP8 pools: bytes into registers ...
+  auto fetch = [&](Raw& rk, Raw& rv) {   // FP8 pools: the bytes of `rows` into registers ...
     if (kSome && tid >= KT * LROW) return;
 #pragma unroll
     for (int e = 0; e < NR; ++e) {
-      const int64_t at = pool_at(step, e);
+      const int64_t at = byte_at(e);
       rk.w[kF8 ? e : 0] = *reinterpret_cast<const u32x4*>(a.k_cache + at);
       rv.w[kF8 ? e : 0] = *reinterpret_cast<const u32x4*>(a.v_cache + at);
     }
@@ -433,7 +464,7 @@ void rows_kernel(Args a) {
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int i = 0; i < 16; ++i) oacc[db][i] = 0.f;
-  float mref = -INFINITY, nmref = kNoRef, lsum = 0.f;
+  float nmref = kNoRef, lsum = 0.f;   // the reference's negative (kNoRef: none yet); P's sum
 
   const int kofs = c32 * RB + ((hf ^ swz<D>(c32)) << 4);
   const int vrow = 4 * hf + ((lane & 15) >> 2);
@@ -453,6 +484,8 @@ void rows_kernel(Args a) {
   // Step i over the K and V tiles kt, vt
   auto step = [&](int i, const char* kt, const char* vt) {
     const int key0 = i * KT;
+    // (products first where waves of a SIMD compete: their operands come from LDS)
+    __builtin_amdgcn_s_setprio(1);
     f32x16 s;   // S^T[key 8 (i/4) + 4 hf + i%4][row c32]
     {
       u32x4 ka[NC];
@@ -467,6 +500,7 @@ void rows_kernel(Args a) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     if constexpr (kCapped == kPlainCap) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -491,11 +525,12 @@ void rows_kernel(Args a) {
     }
     const bool whole = (key0 >= w_lo1 && key0 + KT <= w_hi0) || (key0 >= w_first1 && key0 + KT <= w_pre0);
     if (!whole) {
+      const Keys ks = s_see[wave * 32 + c32];
       const int o = key0 + 4 * hf;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int key = o + 8 * (e >> 2) + (e & 3);
-        const bool seen = (key >= see.lo && key < see.hi) || (key >= see.first && key < see.pre);
+        const bool seen = (key >= ks.lo && key < ks.hi) || (key >= ks.first && key < ks.pre);
         const float x = s[e];
         s[e] = seen ? x : hidden;
       }
@@ -542,17 +577,18 @@ void rows_kernel(Args a) {
         mx = fmaxf(mx, kUnit ? x : fmaf(x, cs, off));
       }
       mx = half_max(mx);
-      const bool nd = mx > mref + Bound<TT>::kMove;
-      const float mnew = nd ? mx + Bound<TT>::kBias : mref;
-      const float alpha = nd ? __builtin_amdgcn_exp2f(mref - mnew) : 1.f;   // 0 from -inf
+      // (without a reference -nmref is below any score, and alpha 0)
+      const bool nd = mx > Bound<TT>::kMove - nmref;
+      const float mnew = mx + Bound<TT>::kBias;
+      const float alpha = nd ? __builtin_amdgcn_exp2f(-nmref - mnew) : 1.f;
 #pragma unroll
       for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
       lsum *= alpha;
-      mref = mnew;
-      nmref = mnew == -INFINITY ? kNoRef : -mnew;
+      nmref = nd ? -mnew : nmref;
       expo();
       if constexpr (kBySum) st = sum_p(0.f);
     }
+    __builtin_amdgcn_s_setprio(1);
     u32x4 va[NPV];
     auto read = [&](int x) {   // 16-key block x / DB, 32-dim block x % DB
       const int at = vofs ^ (x % DB << 6);
@@ -569,9 +605,10 @@ void rows_kernel(Args a) {
     for (int x = 0; x < NPV; ++x) {
       if (x + kAhead < NPV) read(x + kAhead);
       oacc[x % DB] = Mma<TT>::m32(va[x], u32x4{pb[x / DB * 4], pb[x / DB * 4 + 1], pb[x / DB * 4 + 2],
-                                                 pb[x / DB * 4 + 3]}, oacc[x % DB]);
+                                               pb[x / DB * 4 + 3]}, oacc[x % DB]);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
   };
 
   // ---- the part's steps, from the last back: near ones, then far ones, each in
@@ -599,29 +636,45 @@ void rows_kernel(Args a) {
     // would cover the tile loads too
     __builtin_amdgcn_s_waitcnt(kWaitVm0);
     __syncthreads();
+    find_rows(top);
     if constexpr (kF8) {
-      fetch(top, rk, rv);
+      fetch(rk, rv);
       stash(rk, rv, 0);
+      if (N > 1) find_rows(top - 1);
     } else {
-      load(top, 0);
-      if (kBufs > 2 && N > 1) load(top - 1, 1);
+      load(0);
+      if (N > 1) find_rows(top - 1);
+      if (kBufs > 2) {
+        if (N > 1) load(1);
+        if (N > 2) find_rows(top - 2);
+      }
     }
-    int buf = 0;
-    for (int n = 0; n < N; ++n) {
-      const int next = buf == kBufs - 1 ? 0 : buf + 1;
+    // step n over the tiles in buffer `buf` (a constant)
+    auto body = [&](int n, int buf) {
+      constexpr int kFar = kF8 ? 1 : kBufs - 1;   // steps that loads start ahead
       if constexpr (kF8) {
         wait_and_barrier<63>();
-        if (n + 1 < N) fetch(top - n - 1, rk, rv);
+        if (n + kFar < N) fetch(rk, rv);
       } else {
         if (kBufs > 2 && n + 1 < N) wait_and_barrier<2 * NR>();   // tile n + 1 may be in flight
         else wait_and_barrier<0>();
-        if (n + kBufs - 1 < N) load(top - n - (kBufs - 1), buf == 0 ? kBufs - 1 : buf - 1);
+        if (n + kFar < N) load((buf + kBufs - 1) % kBufs);
       }
+      if (n + kFar + 1 < N) find_rows(top - n - kFar - 1);
       step(top - n, s_k + buf * TB, s_v + buf * TB);
       if constexpr (kF8) {
-        if (n + 1 < N) stash(rk, rv, next);
+        if (n + 1 < N) stash(rk, rv, (buf + 1) % kBufs);
       }
-      buf = next;
+    };
+    for (int n = 0; n < N;) {
+      body(n, 0);
+      if (++n >= N) break;
+      body(n, 1);
+      if (++n >= N) break;
+      if constexpr (kBufs > 2) {
+        body(n, 2);
+        ++n;
+      }
     }
   }
 
@@ -639,7 +692,11 @@ void rows_kernel(Args a) {
   const uint32_t bad_rows = (uint32_t)bad | (uint32_t)(bad >> 32);
   const float oscale = kF8 ? a.v_scale[kh] : 1.f;
   const int64_t slot0 = (int64_t)blockIdx.x * TR + wave * 32;
-  if (row_ok && !((bad_rows >> c32) & 1)) {
+  int c = c32;   // (opaque: the row is found again, not kept through the loop)
+  asm volatile("" : "+v"(c));
+  const Row dst = row_of(c);
+  uint16_t* op = a.out + dst.strides(a.out_stride_token, a.out_stride_head);
+  if (dst.ok && !((bad_rows >> c) & 1)) {
     const float inv = ltot > 0.f ? oscale / ltot : 0.f;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -649,14 +706,14 @@ void rows_kernel(Args a) {
         if (e >= d) continue;
         const f32x4 v = f32x4{oacc[db][4 * i], oacc[db][4 * i + 1], oacc[db][4 * i + 2], oacc[db][4 * i + 3]};
         if (merged)
-          *reinterpret_cast<f32x4*>(a.tile_o + (slot0 + c32) * d + e) = v;
+          *reinterpret_cast<f32x4*>(a.tile_o + (slot0 + c) * d + e) = v;
         else
           *reinterpret_cast<u32x2*>(op + e) =
               u32x2{TT::pack2(v.x * inv, v.y * inv), TT::pack2(v.z * inv, v.w * inv)};
       }
     if (merged && hf == 0) {
-      a.tile_ml[(slot0 + c32) * 2] = mref;
-      a.tile_ml[(slot0 + c32) * 2 + 1] = ltot;
+      a.tile_ml[(slot0 + c) * 2] = nmref == kNoRef ? -INFINITY : -nmref;
+      a.tile_ml[(slot0 + c) * 2 + 1] = ltot;
     }
   }
   if (__builtin_expect(bad_rows == 0, 1)) return;
@@ -665,9 +722,10 @@ void rows_kernel(Args a) {
   // keys that the row sees in this part; lane l holds dims 4l .. 4l + 3
   for (int w = 0; w < 32; ++w) {
     if (!((bad_rows >> w) & 1) || f0 + w >= frows) continue;
-    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, w); };
-    const int rlo = of(see.lo), rhi = of(see.hi), rfirst = of(see.first), rpre = of(see.pre);
-    const int rpos = of(pos), rtok = of(qrow), rh = of(h);
+    const Keys ks = s_see[wave * 32 + w];
+    const Row rr = row_of(w);
+    const int rh = rr.h, rpos = a.cu_seqlens_q ? it.limit - it.tokens + rr.tok
+                                               : clampi(a.seq_lens[rr.q], 0, cap_keys) - 1;
     const float rslope = kBias ? a.slopes[rh] * kLog2e : 0.f;
     const int d0 = lane * 4;
     const bool on = d0 < d;
@@ -676,13 +734,12 @@ void rows_kernel(Args a) {
     };
     float qv[4] = {0, 0, 0, 0}, o[4] = {0, 0, 0, 0};
     if (on)
-      widen(*reinterpret_cast<const u32x2*>(a.q + (int64_t)rtok * a.q_stride_token +
-                                            (int64_t)rh * a.q_stride_head + d0), qv);
+      widen(*reinterpret_cast<const u32x2*>(a.q + rr.strides(a.q_stride_token, a.q_stride_head) + d0), qv);
     float m = -INFINITY, l = 0.f;
     for (int i = st0; i < st1; ++i) {
       const int step = i < nfar ? fs0 + i : ns0 + (i - nfar);
       for (int key = step * KT; key < step * KT + KT; ++key) {
-        if (!((key >= rlo && key < rhi) || (key >= rfirst && key < rpre))) continue;
+        if (!((key >= ks.lo && key < ks.hi) || (key >= ks.first && key < ks.pre))) continue;
         const int lb = a.bs_shift >= 0 ? key >> a.bs_shift : key / bs;
         const int bid = clampi(a.block_tables[(int64_t)it.s * a.max_bps + lb], 0, a.num_blocks - 1);
         const int64_t at = ((int64_t)(bid * a.num_kv_heads + kh) * bs + (key - lb * bs)) * rowb + d0 * EB;
@@ -714,8 +771,7 @@ void rows_kernel(Args a) {
     if (!merged) {
       const float inv = l > 0.f || l != l ? oscale / l : 0.f;
       if (on)
-        *reinterpret_cast<u32x2*>(a.out + (int64_t)rtok * a.out_stride_token +
-                                  (int64_t)rh * a.out_stride_head + d0) =
+        *reinterpret_cast<u32x2*>(a.out + rr.strides(a.out_stride_token, a.out_stride_head) + d0) =
             u32x2{TT::pack2(o[0] * inv, o[1] * inv), TT::pack2(o[2] * inv, o[3] * inv)};
     } else {
       const int64_t slot = slot0 + w;
