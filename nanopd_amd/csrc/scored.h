@@ -34,8 +34,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoRef = 3.402823466e38f;   // exponent offset of a row without a reference
 constexpr int kTileRows = 128;              // rows of a workgroup of the rows kernel
 // ... and how many of them run at once on a compute unit at (padded) head dim d
-__host__ __device__ constexpr int rows_per_cu(int64_t d) { return d > 128 ? 1 : d > 64 ? 3 : 4; }
+// (FP8 bytes pass through registers: at three, steps of 128 dims would spill)
+__host__ __device__ constexpr int rows_per_cu(int64_t d, bool fp8) {
+  return d > 128 ? 1 : d > 64 ? (fp8 ? 2 : 3) : 4;
+}
 constexpr int kStepKeys = 32;               // keys per step of the rows kernel
+// Shares of the rows kernel's workgroups, in steps: what a piece of a tile costs
+// besides its steps, the smallest share (but for its tilt), and how near a tile's edge no cut is made.
+constexpr int kTileCost = 6;
+constexpr int kMinShare = 16;
+constexpr int kNearEdge = 4;
 constexpr int kListTiles = 512;             // most tiles per kv head that are cut into parts
 constexpr int kUnitHeads = 16;              // most heads of a stream unit (MFMA columns)
 
@@ -55,9 +63,9 @@ struct Args {
   const float* v_scale;
   const int32_t* cu_groups;       // shared prefixes: sequences of group g are
   const int32_t* shared_lens;     // cu_groups[g] .. cu_groups[g + 1] - 1
-  float* tile_o;                  // partials of the rows kernel [item][kv head][row][D]
+  float* tile_o;                  // partials of the rows kernel [slot][kv head][row][D]
   float* tile_ml;                 // their (m, l)
-  int32_t* tile_items;            // [tile][kv head]: first item and parts
+  int32_t* tile_items;            // [tile][kv head][4]: first slot, first and last workgroup
   float* unit_o;                  // partials of the stream kernel [seq][head][part][D]
   float* unit_ml;
   int num_seqs, num_groups, total_q, max_shared;
@@ -65,8 +73,10 @@ struct Args {
   int block_size, bs_shift, num_blocks, max_bps;   // bs_shift < 0: no power of two
   int tiles;                      // rows kernel: tiles of all sequences or groups
   int tiles_max;                  // ... chunks: most tiles of one sequence
-  int items, room;                // ... items per kv head, and those that run at once
-  bool list;                      // ... tiles are cut into parts (else one item each)
+  int room;                       // ... workgroups per kv head (chunks without a list: whole tiles)
+  int room1;                      // ... of them in one round over the compute units
+  bool list;                      // ... that share the steps of all tiles evenly
+  int cost_shift;                 // ... whose cost is counted in 2^shift steps
   int unit_splits;                // stream kernel: most parts of a unit
   int subs, sub_heads;            // stream kernel: units per kv head, heads of a unit
   int window;                     // 0: none
@@ -130,9 +140,8 @@ __device__ __forceinline__ Group group_at(const Args& a, int g) {
   r.tile0 = 0;
   return r;
 }
-// kBySeq: of the group that holds sequence x, else of the one that holds tile x.
-// false: none.
-template <bool kBySeq>
+// The group that holds sequence x (its first tile of the rows kernel too). false:
+// none.
 __device__ __forceinline__ bool find_group(const Args& a, int x, int lane, Group& out) {
   int base = 0;
   for (int g0 = 0; g0 < a.num_groups; g0 += 64) {
@@ -144,8 +153,7 @@ __device__ __forceinline__ bool find_group(const Args& a, int x, int lane, Group
     }
     const int incl = wave_scan_i(n);
     const int t0 = base + incl - n;
-    const bool hit = kBySeq ? x >= r.seq0 && x < r.seq0 + r.seqs : x >= t0 && x < t0 + n;
-    const uint64_t m = __ballot(hit);
+    const uint64_t m = __ballot(x >= r.seq0 && x < r.seq0 + r.seqs);
     if (m != 0) {
       const int sel = __builtin_ctzll(m);
       out.seq0 = __builtin_amdgcn_readlane(r.seq0, sel);
@@ -214,12 +222,10 @@ __device__ __forceinline__ u32x4 e4m3x8_to(uint32_t lo, uint32_t hi) {
                e4m3x2_to<TT, true>(hi)};
 }
 
-// Launchers (scored_rows_*.hip, scored_stream.hip).
+// Launcher by padded head dim (scored_rows_d*.hip): chunks, or groups (the shared
+// keys and the sequences' own ones in one launch).
 template <int D>
 void launch_rows(const Args& a, int32_t dtype, hipStream_t st);
-extern template void launch_rows<64>(const Args&, int32_t, hipStream_t);
-extern template void launch_rows<128>(const Args&, int32_t, hipStream_t);
-extern template void launch_rows<256>(const Args&, int32_t, hipStream_t);
 
 }  // namespace scored
 }  // namespace npd

@@ -1,349 +1,155 @@
-// Decode attention with changed scores (scored.h): the kernel that streams the
-// keys of one token per sequence, the merge of partial results, and the C
-// entries of the scored attention ops.
-//
-// Work unit: one wave per (sequence, kv head, up to 16 of its query heads, part
-// of the keys that the token sees). All heads of a unit see the same keys, so
-// masks are no part of the loop: the keys seen are two ranges (prefix and own
-// range), taken as one list of pool rows in LDS, which also makes any block size,
-// window start and head dim one path. Per step of 16 keys:
-//   S^T = K . Q^T on v_mfma_f32_16x16x32, K read from the pool in its operand
-//     layout (16 bytes per lane, the heads padded to 16 columns);
-//   the head's reference moves only when a step's maximum passes it by 2^8;
-//   O^T += V^T . P^T on v_mfma_f32_16x16x16, V through LDS for the transposing
-//     reads of its operand.
-// Loads run kRing steps ahead in registers (about 16 KB of a wave in flight at
-// any head dim). Bound: HBM, the unit's K/V bytes.
-// Parts: a unit's keys are cut into near-equal parts of at least kMinPart keys,
-// as many as the launch has waves for it (unit_splits), from the lengths on the
-// device; the parts meet in the merge kernel.
-#include "scored.h"
+// Attention with changed scores over the paged pool: the C entries, the decode
+// kernel (units of scored_stream.h) and the merges of partial results.
+#include "scored_stream.h"
 
 namespace npd {
 namespace scored {
 namespace {
 
-constexpr int kListKeys = 1024;      // rows listed in LDS at a time (a multiple of every ring)
-constexpr int kMinPart = 256;        // shortest part of a unit (keys)
-constexpr float kTau = 8.f;          // a reference moves by more than this (log2 units)
-constexpr int kTargetItems = 4096;   // waves of a launch, about
+constexpr int kTargetItems = 4096;   // waves of a stream launch, about
 
-// Nontemporal: a pool row is read once per call (by one unit per kv head).
-__device__ __forceinline__ u32x4 ld_stream(const char* p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-}
-
-// Keys of sequence s that its stream units take (past the shared ones).
-__device__ __forceinline__ void unit_keys(const Args& a, int s, int lane, int& pos, int& a0, int& na,
-                                          int& b0, int& nb) {
-  const int ctx = clampi(a.seq_lens[s], 0, a.max_bps * a.block_size);
-  pos = ctx - 1;
-  const Keys k = row_keys(pos, ctx, a.first_keys ? a.first_keys[s] : 0,
-                          a.prefix_lens ? a.prefix_lens[s] : 0, a.window);
-  int from = 0;
-  if (a.cu_groups) {
-    Group g;
-    if (find_group<true>(a, s, lane, g)) from = g.shared;
-  }
-  b0 = k.lo < from ? from : k.lo;
-  nb = k.hi > b0 ? k.hi - b0 : 0;
-  a0 = k.first < from ? from : k.first;
-  const int ae = k.pre < b0 ? k.pre : b0;
-  na = ae > a0 ? ae - a0 : 0;
-  // prefix keys past the token: none (pre <= context = position + 1)
-}
-__device__ __forceinline__ int unit_parts(const Args& a, int keys) {
-  const int p = (keys + kMinPart - 1) / kMinPart;
-  return p < a.unit_splits ? p : a.unit_splits;
-}
-
-// DP: the head dim padded to 64, 128 or 256. Chunks past the row's end load its
-// last chunk against zero queries; their output dims are not stored.
 template <class TT, int DP, bool kF8>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2)))
 void stream_kernel(Args a) {
-  constexpr int kRing = DP == 64 || (kF8 && DP == 128) ? 4 : (DP == 128 || kF8 ? 2 : 1);
-  constexpr int EB = kF8 ? 1 : 2;                  // bytes per element
-  constexpr int CPR = DP * EB / 16;                // 16-byte chunks per (padded) row
-  constexpr int NKL = CPR / 4;                     // K loads per lane and step
-  constexpr int TPL = 64 / CPR;                    // rows per V load
-  constexpr int NVL = 16 / TPL;                    // V loads per lane and step
-  constexpr int NKC = DP / 32;                     // S MFMAs per step
-  constexpr int NOB = DP / 16;                     // 16-dim blocks of O^T
-  constexpr int VROW = DP + 16;                    // V row in LDS: an 8-bank shift per row
-  static_assert(NKL >= 1 && NVL >= 1, "row shape");
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[16 * VROW];
-  __shared__ int s_row[kListKeys];
-  const int lane = threadIdx.x, g4 = lane >> 4, n16 = lane & 15;
-  const int units = a.num_seqs * a.num_kv_heads * a.subs;
-  const int part = (int)blockIdx.x / units, unit = (int)blockIdx.x - part * units;
-  const int sub = unit % a.subs, kh = unit / a.subs % a.num_kv_heads;
-  const int s = unit / a.subs / a.num_kv_heads;
-  const int h0 = kh * a.group + sub * a.sub_heads;
-  const int heads = min(a.sub_heads, a.group - sub * a.sub_heads);
-  const int d = a.head_dim;
-
-  int pos, a0, na, b0, nb;
-  unit_keys(a, s, lane, pos, a0, na, b0, nb);
-  const int keys = na + nb;
-  const int parts = unit_parts(a, keys);
-  const bool direct = !a.cu_groups && parts <= 1;
-  uint16_t* orow = a.out + s * a.out_stride_token + (h0 + n16) * a.out_stride_head;
-  if (part >= parts) {
-    if (part == 0 && direct && n16 < heads)   // no key at all: zero rows
-      for (int e = g4 * 4; e < d; e += 16) *reinterpret_cast<u32x2*>(orow + e) = u32x2{0, 0};
-    return;
-  }
-  const int span = ((keys + parts - 1) / parts + 15) / 16 * 16;
-  const int k0 = part * span < keys ? part * span : keys;
-  const int k1 = k0 + span < keys ? k0 + span : keys;
-
-  // Q^T as the B operand: lane (g4, n16) = head n16, the dims of the K operand
-  // (2-byte pools: chunk c = dims 32c + 8 g4 ..; FP8: load c covers dims 64c +
-  // 16 g4 .., converted in two halves)
-  u32x4 qb[NKC];
-  {
-    const uint16_t* qrow = a.q + s * a.q_stride_token + (h0 + n16) * a.q_stride_head;
-#pragma unroll
-    for (int c = 0; c < NKC; ++c) {
-      const int at = kF8 ? 64 * (c / 2) + 16 * g4 + 8 * (c % 2) : 32 * c + 8 * g4;
-      qb[c] = n16 < heads && at < d ? *reinterpret_cast<const u32x4*>(qrow + at) : u32x4{0, 0, 0, 0};
-    }
-  }
-  const float kscale = kF8 ? a.k_scale[kh] : 1.f;
-  const float oscale = kF8 ? a.v_scale[kh] : 1.f;
-  const bool cap = a.cap_log2 > 0.f;
-  const float c2 = a.scale_log2 * kscale, cin = a.cap_in * kscale;
-  const float slope = a.slopes && n16 < heads ? a.slopes[h0 + n16] * kLog2e : 0.f;
-  const int64_t rowb = (int64_t)d * EB;
-  const int last = (int)(rowb / 16) - 1;            // the row's last chunk
-  const int j = lane % CPR, r = lane / CPR;         // V: chunk and row of this lane's loads
-  const int vcol = (j < last ? j : last) * 16;
-  int kcol[NKL];
-#pragma unroll
-  for (int c = 0; c < NKL; ++c) kcol[c] = (4 * c + g4 < last ? 4 * c + g4 : last) * 16;
-
-  f32x4 oacc[NOB];
-#pragma unroll
-  for (int b = 0; b < NOB; ++b) oacc[b] = f32x4{0, 0, 0, 0};
-  float mref = -INFINITY, lp = 0.f;   // head n16's reference; this lane's sum of its P
-  const uint16_t* vl = s_v + (g4 * 4 + (n16 >> 2)) * VROW + 4 * (n16 & 3);
-
-  for (int t0 = k0; t0 < k1; t0 += kListKeys) {
-    const int ntok = k1 - t0 < kListKeys ? k1 - t0 : kListKeys;
-    const int nsteps = ((ntok + 15) / 16 + kRing - 1) / kRing * kRing;
-    // pool rows of the keys; entries past them repeat the last one
-    __syncthreads();
-    for (int e = lane; e < nsteps * 16; e += 64) {
-      const int x = t0 + (e < ntok ? e : ntok - 1);
-      const int key = x < na ? a0 + x : b0 + (x - na);
-      const int lb = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
-      const int bid = clampi(a.block_tables[(int64_t)s * a.max_bps + lb], 0, a.num_blocks - 1);
-      s_row[e] = (bid * a.num_kv_heads + kh) * a.block_size + (key - lb * a.block_size);
-    }
-    __syncthreads();
-    auto load_k = [&](u32x4* buf, int st) {
-      const char* p = a.k_cache + (int64_t)s_row[st * 16 + n16] * rowb;
-#pragma unroll
-      for (int c = 0; c < NKL; ++c) buf[c] = ld_stream(p + kcol[c]);
-    };
-    auto load_v = [&](u32x4* buf, int st) {
-#pragma unroll
-      for (int i = 0; i < NVL; ++i)
-        buf[i] = ld_stream(a.v_cache + (int64_t)s_row[st * 16 + i * TPL + r] * rowb + vcol);
-    };
-    auto step = [&](const u32x4* kraw, const u32x4* vraw, int st) {
-      // V rows into LDS; past the last key zeros, so that an infinity there
-      // meets no zero probability
-      const bool tail = st * 16 + 16 > ntok;
-#pragma unroll
-      for (int i = 0; i < NVL; ++i) {
-        const int row = i * TPL + r;
-        u32x4 v = vraw[i];
-        if (tail && st * 16 + row >= ntok) v = u32x4{0, 0, 0, 0};
-        if constexpr (kF8) {
-          *reinterpret_cast<u32x4*>(&s_v[row * VROW + j * 16]) = e4m3x8_to<TT>(v.x, v.y);
-          *reinterpret_cast<u32x4*>(&s_v[row * VROW + j * 16 + 8]) = e4m3x8_to<TT>(v.z, v.w);
-        } else {
-          *reinterpret_cast<u32x4*>(&s_v[row * VROW + j * 8]) = v;
-        }
-      }
-      f32x4 sacc = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int c = 0; c < NKL; ++c) {
-        if constexpr (kF8) {
-          sacc = Mma<TT>::k32(e4m3x8_to<TT>(kraw[c].x, kraw[c].y), qb[2 * c], sacc);
-          sacc = Mma<TT>::k32(e4m3x8_to<TT>(kraw[c].z, kraw[c].w), qb[2 * c + 1], sacc);
-        } else {
-          sacc = Mma<TT>::k32(kraw[c], qb[c], sacc);
-        }
-      }
-      float sv[4];
-      const int e0 = st * 16 + 4 * g4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sv[i] = cap ? cap_exact(sacc[i], cin, a.cap_log2) : sacc[i] * c2;
-      if (a.slopes) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int x = t0 + e0 + i;
-          const int key = x < na ? a0 + x : b0 + (x - na);
-          sv[i] = fmaf(-slope, (float)(pos - key), sv[i]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sv[i] = e0 + i < ntok ? sv[i] : -INFINITY;
-      const float x = row_max4(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])));
-      float f = 1.f;
-      if (x > mref + kTau) {
-        f = mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - x);
-        mref = x;
-      }
-      if (__ballot(f != 1.f) != 0) {   // the first step, then rarely
-        lp *= f;
-#pragma unroll
-        for (int b = 0; b < NOB; ++b) oacc[b] *= f;
-      }
-      const float ref = mref == -INFINITY ? 0.f : mref;
-      const uint32_t p01 = TT::pack2(__builtin_amdgcn_exp2f(sv[0] - ref), __builtin_amdgcn_exp2f(sv[1] - ref));
-      const uint32_t p23 = TT::pack2(__builtin_amdgcn_exp2f(sv[2] - ref), __builtin_amdgcn_exp2f(sv[3] - ref));
-      lp += (TT::lo(p01) + TT::hi(p01)) + (TT::lo(p23) + TT::hi(p23));
-      const u32x2 pb = u32x2{p01, p23};
-#pragma unroll
-      for (int b = 0; b < NOB; ++b) oacc[b] = Mma<TT>::k16(lds_read_tr(vl + b * 16), pb, oacc[b]);
-    };
-    u32x4 kb[kRing][NKL], vb[kRing][NVL];
-#pragma unroll
-    for (int b = 0; b < kRing; ++b) {
-      load_k(kb[b], b);
-      load_v(vb[b], b);
-    }
-    int st0 = 0;
-    for (; st0 + kRing < nsteps; st0 += kRing) {
-#pragma unroll
-      for (int b = 0; b < kRing; ++b) {
-        step(kb[b], vb[b], st0 + b);
-        load_k(kb[b], st0 + kRing + b);
-        load_v(vb[b], st0 + kRing + b);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < kRing; ++b) step(kb[b], vb[b], st0 + b);
-  }
-  const float lsum = row_sum4(lp);
-  if (n16 >= heads) return;
-  if (direct) {
-    const float inv = lsum > 0.f || lsum != lsum ? oscale / lsum : 0.f;
-#pragma unroll
-    for (int b = 0; b < NOB; ++b)
-      if (b * 16 + 4 * g4 < d)
-        *reinterpret_cast<u32x2*>(orow + b * 16 + 4 * g4) =
-            u32x2{TT::pack2(oacc[b].x * inv, oacc[b].y * inv), TT::pack2(oacc[b].z * inv, oacc[b].w * inv)};
-    return;
-  }
-  const int64_t slot = ((int64_t)s * a.num_heads + h0 + n16) * a.unit_splits + part;
-#pragma unroll
-  for (int b = 0; b < NOB; ++b)
-    if (b * 16 + 4 * g4 < d) *reinterpret_cast<f32x4*>(a.unit_o + slot * d + b * 16 + 4 * g4) = oacc[b];
-  if (g4 == 0) {
-    a.unit_ml[slot * 2] = mref;
-    a.unit_ml[slot * 2 + 1] = lsum;
-  }
+  __shared__ __attribute__((aligned(16))) StreamLds<DP> lds;
+  stream_unit<TT, DP, kF8>(a, blockIdx.x, threadIdx.x, lds);
 }
 
-// Merge: one wave per (token, head) row. The row's partials are the parts of its
-// stream units and, with groups, of its group's tiles (chunks: of its tile).
-// LPR lanes hold four dims each; the 64 / LPR lane groups take slots in turn.
-template <class TT, int LPR>
-__global__ __launch_bounds__(256) void merge_kernel(Args a) {
-  constexpr int SG = 64 / LPR;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int h = (int)(row % a.num_heads);
-  const int tok = (int)(row / a.num_heads);
-  if (tok >= a.total_q) return;
-  const int kh = h / a.group, hh = h - kh * a.group, d = a.head_dim;
-  int nt = 0, nu = 0;        // partials of tiles and of stream units
-  int64_t tslot = 0, uslot = 0;
-  const int64_t tstep = (int64_t)a.num_kv_heads * kTileRows;   // slots between a tile's parts
-  if (a.cu_seqlens_q) {
-    // the sequence of the token: the last that starts at or before it (binary search)
-    int lo = 0, hi = a.num_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.cu_seqlens_q[mid] <= tok) lo = mid; else hi = mid - 1;
-    }
-    const int q0 = clampi(a.cu_seqlens_q[lo], 0, a.total_q);
-    const int q1 = clampi(a.cu_seqlens_q[lo + 1], q0, a.total_q);
-    if (tok < q0 || tok >= q1) return;
-    const int f = (tok - q0) * a.group + hh;
-    if (f / kTileRows >= a.tiles_max) return;
-    const int64_t tile = (int64_t)q0 * a.group / kTileRows + lo + f / kTileRows;
-    const int32_t* ti = a.tile_items + 2 * (tile * a.num_kv_heads + kh);
-    nt = ti[1];
-    if (nt <= 1) return;     // written by the rows kernel itself
-    tslot = ((int64_t)ti[0] * a.num_kv_heads + kh) * kTileRows + f % kTileRows;
-  } else {
-    int pos, a0, na, b0, nb;
-    unit_keys(a, tok, lane, pos, a0, na, b0, nb);
-    nu = unit_parts(a, na + nb);
-    if (!a.cu_groups && nu <= 1) return;   // written by the stream kernel itself
-    uslot = ((int64_t)tok * a.num_heads + h) * a.unit_splits;
-    Group g;
-    if (a.cu_groups && find_group<true>(a, tok, lane, g) && g.shared > 0) {
-      const int64_t f = (int64_t)(tok - g.seq0) * a.group + hh;
-      const int64_t tile = g.tile0 + f / kTileRows;
-      if (tile < a.tiles) {
-        const int32_t* ti = a.tile_items + 2 * (tile * a.num_kv_heads + kh);
-        nt = ti[1];
-        tslot = ((int64_t)ti[0] * a.num_kv_heads + kh) * kTileRows + f % kTileRows;
-      }
-    }
+// Partials of a row: `nt` of its tile (slot t0 and then every second from t1 on,
+// tstep apart) and `nu` of its stream units (consecutive from u0).
+struct Parts {
+  int nt, nu;
+  int64_t t0, t1, tstep, u0;
+  __device__ __forceinline__ bool tile(int i) const { return i < nt; }
+  __device__ __forceinline__ int64_t slot(int i) const {
+    return i >= nt ? u0 + (i - nt) : i == 0 ? t0 : t1 + i * tstep;
   }
-  // (lists that do not ascend may leave an entry unwritten: stay in the buffer)
-  const int64_t room = (int64_t)a.items * a.num_kv_heads * kTileRows;
-  if (tslot < 0 || nt < 0 || tslot + nt * tstep > room + tstep - kTileRows) nt = 0;
-  const int n = nt + nu;
-  auto ml = [&](int i) {
-    return i < nt ? a.tile_ml + (tslot + i * tstep) * 2 : a.unit_ml + (uslot + i - nt) * 2;
-  };
-  auto ov = [&](int i) {
-    return i < nt ? a.tile_o + (tslot + i * tstep) * d : a.unit_o + (uslot + i - nt) * d;
-  };
+};
+// The merge of a row by LPR lanes (four dims each), every part's sum weighted by
+// 2^(m - M); kFlight parts' loads at a time.
+template <class TT, int LPR>
+__device__ __forceinline__ void merge_row(const Args& a, const Parts& p, int lane, uint16_t* dst,
+                                          float oscale) {
+  constexpr int kFlight = 4;
+  const int n = p.nt + p.nu, d = a.head_dim, j = lane % LPR, c = j * 4;
+  auto ml = [&](int i) { return (p.tile(i) ? a.tile_ml : a.unit_ml) + p.slot(i) * 2; };
   float M = -INFINITY;
-  for (int i = lane; i < n; i += 64) M = fmaxf(M, ml(i)[0]);
-  M = wave_max_f(M);
-  const int c = (lane % LPR) * 4;
+  for (int i = j; i < n; i += LPR) M = fmaxf(M, ml(i)[0]);
+#pragma unroll
+  for (int k = 1; k < LPR; k <<= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
   f32x4 o = f32x4{0, 0, 0, 0};
   float L = 0.f;
   if (M > -INFINITY) {
-    for (int i = lane / LPR; i < n; i += SG) {
-      const float* p = ml(i);
-      if (p[0] == -INFINITY) continue;   // a part without a key
-      const float w = __builtin_amdgcn_exp2f(p[0] - M);
-      L = fmaf(p[1], w, L);
-      if (c < d) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(ov(i) + c);
-        o.x = fmaf(x.x, w, o.x);
-        o.y = fmaf(x.y, w, o.y);
-        o.z = fmaf(x.z, w, o.z);
-        o.w = fmaf(x.w, w, o.w);
+    for (int i0 = 0; i0 < n; i0 += kFlight) {
+      float w[kFlight], l[kFlight];
+      f32x4 x[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const int i = i0 + k < n ? i0 + k : n - 1;
+        const float* q = ml(i);
+        w[k] = i0 + k < n ? q[0] : -INFINITY;
+        l[k] = q[1];
+        x[k] = f32x4{0, 0, 0, 0};
+        // (a part without a key has no sums)
+        if (w[k] != -INFINITY && c < d)
+          x[k] = *reinterpret_cast<const f32x4*>((p.tile(i) ? a.tile_o : a.unit_o) + p.slot(i) * d + c);
+      }
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const float f = __builtin_amdgcn_exp2f(w[k] - M);
+        if (w[k] != -INFINITY) L = fmaf(l[k], f, L);
+        o.x = fmaf(x[k].x, f, o.x);
+        o.y = fmaf(x[k].y, f, o.y);
+        o.z = fmaf(x[k].z, f, o.z);
+        o.w = fmaf(x[k].w, f, o.w);
       }
     }
   }
-#pragma unroll
-  for (int k = LPR; k < 64; k <<= 1) {
-    L += __shfl_xor(L, k, 64);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float v = o[e];
-      o[e] = v + __shfl_xor(v, k, 64);
-    }
-  }
-  if (lane < LPR && c < d) {
-    const float inv = L > 0.f || L != L ? (a.v_scale ? a.v_scale[kh] : 1.f) / L : 0.f;
-    uint16_t* dst = a.out + tok * a.out_stride_token + h * a.out_stride_head + c;
-    *reinterpret_cast<u32x2*>(dst) =
+  if (c < d) {
+    const float inv = L > 0.f || L != L ? oscale / L : 0.f;
+    *reinterpret_cast<u32x2*>(dst + c) =
         u32x2{TT::pack2(o.x * inv, o.y * inv), TT::pack2(o.z * inv, o.w * inv)};
+  }
+}
+
+// A tile's entry as the parts of its row r (none where lists that do not ascend
+// left no such entry: stay in the buffer).
+__device__ __forceinline__ void tile_parts(const Args& a, int64_t tile, int kh, int r, Parts& p) {
+  const int32_t* e = a.tile_items + 4 * (tile * a.num_kv_heads + kh);
+  const int slot0 = e[0], wg = e[1], parts = e[2] - wg + 1;
+  p.nt = 0;
+  if (parts < 1 || parts > a.room || wg < 0 || wg + parts > a.room || slot0 < 0 ||
+      slot0 >= 2 * a.room + a.tiles)
+    return;
+  p.nt = parts;
+  p.t0 = ((int64_t)slot0 * a.num_kv_heads + kh) * kTileRows + r;
+  p.t1 = ((int64_t)2 * wg * a.num_kv_heads + kh) * kTileRows + r;
+  p.tstep = (int64_t)2 * a.num_kv_heads * kTileRows;
+}
+
+// One token per sequence: a wave takes 64 / LPR heads of a token.
+template <class TT, int LPR>
+__global__ __launch_bounds__(256) void merge_tokens_kernel(Args a) {
+  constexpr int R = 64 / LPR;
+  const int lane = threadIdx.x & 63;
+  const int per = (a.num_heads + R - 1) / R;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int s = (int)(w / per), h = (int)(w - (int64_t)s * per) * R + lane / LPR;
+  if (s >= a.num_seqs) return;   // whole waves
+  int pos, a0, na, b0, nb;
+  unit_keys(a, s, lane, pos, a0, na, b0, nb);
+  Parts p{};
+  p.nu = unit_parts(a, na + nb);
+  if (!a.cu_groups && p.nu <= 1) return;   // written by the stream kernel itself
+  Group g;
+  const bool grouped = a.cu_groups && find_group(a, s, lane, g) && g.shared > 0;
+  if (h >= a.num_heads) return;
+  const int kh = h / a.group;
+  p.u0 = ((int64_t)s * a.num_heads + h) * a.unit_splits;
+  if (grouped) {
+    const int64_t f = (int64_t)(s - g.seq0) * a.group + (h - kh * a.group);
+    const int64_t tile = g.tile0 + f / kTileRows;
+    if (tile < a.tiles) tile_parts(a, tile, kh, (int)(f % kTileRows), p);
+  }
+  merge_row<TT, LPR>(a, p, lane, a.out + s * a.out_stride_token + h * a.out_stride_head,
+                     a.v_scale ? a.v_scale[kh] : 1.f);
+}
+
+// Chunks: a workgroup takes a tile's rows of one kv head, kSlice of them.
+constexpr int kSlice = 16;
+template <class TT, int LPR>
+__global__ __launch_bounds__(256) void merge_tiles_kernel(Args a) {
+  const int lane = threadIdx.x & 63;
+  int id = blockIdx.x;
+  const int slice = id % (kTileRows / kSlice);
+  id /= kTileRows / kSlice;
+  const int kh = id % a.num_kv_heads;
+  const int64_t tile = id / a.num_kv_heads;
+  // the sequence: the last whose first tile is at or before this one
+  auto first = [&](int s) {
+    return (int64_t)clampi(a.cu_seqlens_q[s], 0, a.total_q) * a.group / kTileRows + s;
+  };
+  int lo = 0, hi = a.num_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first(mid) <= tile) lo = mid; else hi = mid - 1;
+  }
+  const int q0 = clampi(a.cu_seqlens_q[lo], 0, a.total_q);
+  const int q1 = clampi(a.cu_seqlens_q[lo + 1], q0, a.total_q);
+  const int64_t t = tile - first(lo);
+  const int64_t rows = (int64_t)(q1 - q0) * a.group;
+  if (t < 0 || t >= a.tiles_max || t * kTileRows >= rows) return;
+  const float oscale = a.v_scale ? a.v_scale[kh] : 1.f;
+  for (int r = slice * kSlice + threadIdx.x / LPR; r < (slice + 1) * kSlice; r += 256 / LPR) {
+    const int64_t f = t * kTileRows + r;
+    if (f >= rows) break;
+    Parts p{};
+    tile_parts(a, tile, kh, r, p);
+    if (p.nt <= 1) return;     // written by the rows kernel itself
+    const int64_t tok = f / a.group;
+    const int h = kh * a.group + (int)(f - tok * a.group);
+    merge_row<TT, LPR>(a, p, lane, a.out + (q0 + tok) * a.out_stride_token + h * a.out_stride_head,
+                       oscale);
   }
 }
 
@@ -362,17 +168,26 @@ void launch_stream(const Args& a, hipStream_t st) {
   else if (a.head_dim <= 128) launch_stream_d<TT, 128>(a, items, st);
   else launch_stream_d<TT, 256>(a, items, st);
 }
-template <class TT>
-void launch_merge(const Args& a, hipStream_t st) {
-  const dim3 g((unsigned)(((int64_t)a.total_q * a.num_heads + 3) / 4)), b(256);
-  if (a.head_dim <= 64) hipLaunchKernelGGL((merge_kernel<TT, 16>), g, b, 0, st, a);
-  else if (a.head_dim <= 128) hipLaunchKernelGGL((merge_kernel<TT, 32>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((merge_kernel<TT, 64>), g, b, 0, st, a);
+template <class TT, int LPR>
+void launch_merge_d(const Args& a, hipStream_t st) {
+  if (a.cu_seqlens_q) {
+    const int64_t n = (int64_t)a.tiles * a.num_kv_heads * (kTileRows / kSlice);
+    hipLaunchKernelGGL((merge_tiles_kernel<TT, LPR>), dim3((unsigned)n), dim3(256), 0, st, a);
+  } else {
+    constexpr int R = 64 / LPR;
+    const int64_t waves = (int64_t)a.num_seqs * ((a.num_heads + R - 1) / R);
+    hipLaunchKernelGGL((merge_tokens_kernel<TT, LPR>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a);
+  }
 }
-void launch_rows_any(const Args& a, int32_t dtype, hipStream_t st) {
-  if (a.head_dim <= 64) launch_rows<64>(a, dtype, st);
-  else if (a.head_dim <= 128) launch_rows<128>(a, dtype, st);
-  else launch_rows<256>(a, dtype, st);
+template <class TT>
+void launch_merge_t(const Args& a, hipStream_t st) {
+  if (a.head_dim <= 64) launch_merge_d<TT, 16>(a, st);
+  else if (a.head_dim <= 128) launch_merge_d<TT, 32>(a, st);
+  else launch_merge_d<TT, 64>(a, st);
+}
+void launch_merge(const Args& a, int32_t dtype, hipStream_t st) {
+  if (dtype == NPD_DTYPE_BF16) launch_merge_t<BF16>(a, st);
+  else launch_merge_t<F16>(a, st);
 }
 
 // Units of at most kUnitHeads heads: the fewest near-equal ones.
@@ -388,8 +203,8 @@ int64_t unit_splits_of(int64_t units, int64_t max_keys) {
 }
 
 // Workgroups of the rows kernel that run at once per kv head.
-int64_t rows_room(int64_t head_dim, int64_t num_kv_heads) {
-  const int64_t n = rows_per_cu(head_dim) * (int64_t)device_cus() / num_kv_heads;
+int64_t rows_room(int64_t head_dim, int64_t num_kv_heads, bool fp8) {
+  const int64_t n = rows_per_cu(head_dim, fp8) * (int64_t)device_cus() / num_kv_heads;
   return n < 1 ? 1 : n;
 }
 
@@ -399,11 +214,12 @@ int64_t pad256(int64_t x) { return (x + 255) / 256 * 256; }
 // ops leave alone, so that one buffer serves every attention op), then the
 // tiles' partials and part counts, then the units'.
 struct Plan {
-  int64_t tiles = 0, tiles_max = 0, items = 0, room = 1, unit_splits = 1;
+  int cost_shift = 0;
+  int64_t tiles = 0, tiles_max = 0, room = 1, unit_splits = 1;
   bool list = false;
   int64_t tile_slots = 0, unit_slots = 0, head_dim = 0, kv_heads = 0;
   int64_t tile_items_at() const { return kCounterBytes; }
-  int64_t tile_o_at() const { return tile_items_at() + (tile_slots ? pad256(tiles * kv_heads * 8) : 0); }
+  int64_t tile_o_at() const { return tile_items_at() + (tile_slots ? pad256(tiles * kv_heads * 16) : 0); }
   int64_t tile_ml_at() const { return tile_o_at() + pad256(tile_slots * head_dim * 4); }
   int64_t unit_o_at() const { return tile_ml_at() + pad256(tile_slots * 8); }
   int64_t unit_ml_at() const { return unit_o_at() + pad256(unit_slots * head_dim * 4); }
@@ -424,18 +240,24 @@ Plan decode_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int6
   p.unit_slots = p.unit_splits > 1 ? num_seqs * num_heads * p.unit_splits : 0;
   return p;
 }
+// Slots of the rows kernel's partials: two per workgroup (its first tile may have
+// begun before it and its last may go on after it); groups also one per tile (the
+// parts of whole tiles meet those of the stream units).
+// Shares over at most `tiles` tiles of a kv head with at most `steps` steps each.
+void plan_list(Plan& p, int64_t tiles, int64_t steps) {
+  const int64_t total = tiles * (steps + kTileCost), most = (total + kMinShare - 1) / kMinShare;
+  p.list = true;
+  p.room = p.room < most ? p.room : most < 1 ? 1 : most;
+  while (((steps + kTileCost) >> p.cost_shift) + 1 > (INT32_MAX / 2) / tiles) ++p.cost_shift;
+}
 Plan shared_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                  int64_t max_keys, int64_t num_groups, int64_t max_shared) {
   Plan p = decode_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_keys);
   p.unit_slots = num_seqs * num_heads * p.unit_splits;   // always merged
   p.tiles = num_seqs * (num_heads / num_kv_heads) / kTileRows + num_groups;
-  p.list = true;
-  p.room = rows_room(head_dim, num_kv_heads);
-  // parts of target steps: at most room + one round-up per tile, nor more than
-  // the shared keys' steps
-  const int64_t most = p.tiles * (max_shared / kStepKeys + 1);
-  p.items = p.room + p.tiles < most ? p.room + p.tiles : most;
-  p.tile_slots = p.items * num_kv_heads * kTileRows;
+  p.room = rows_room(head_dim, num_kv_heads, false);
+  plan_list(p, p.tiles, max_shared / kStepKeys + 1);
+  p.tile_slots = (2 * p.room + p.tiles) * num_kv_heads * kTileRows;
   return p;
 }
 Plan chunk_plan(int64_t num_seqs, int64_t total_q, int64_t num_heads, int64_t num_kv_heads,
@@ -446,15 +268,14 @@ Plan chunk_plan(int64_t num_seqs, int64_t total_q, int64_t num_heads, int64_t nu
   p.kv_heads = num_kv_heads;
   p.tiles = total_q * g / kTileRows + num_seqs;
   p.tiles_max = (max_q_len * g + kTileRows - 1) / kTileRows;
-  p.room = rows_room(head_dim, num_kv_heads);
-  p.items = num_seqs * p.tiles_max;
-  const int64_t most = p.tiles < p.items ? p.tiles : p.items;
-  // cut into parts unless whole tiles fill the chip three times over, or hold so
-  // few keys that none would be cut
-  p.list = p.items <= kListTiles && most < 3 * p.room && max_keys > 8 * kStepKeys;
-  if (p.list) {
-    p.items = p.room + most;
-    p.tile_slots = p.items * num_kv_heads * kTileRows;
+  p.room = rows_room(head_dim, num_kv_heads, false);
+  const int64_t all = num_seqs * p.tiles_max, most = p.tiles < all ? p.tiles : all;
+  // shared out evenly unless whole tiles fill the chip twice over
+  if (all <= kListTiles && most < 2 * p.room) {
+    plan_list(p, most, max_keys / kStepKeys + 2);
+    p.tile_slots = p.room > 1 ? 2 * p.room * num_kv_heads * kTileRows : 0;
+  } else {
+    p.room = all;
   }
   return p;
 }
@@ -565,9 +386,14 @@ Args make_args(const Call& c, const Plan& p, void* workspace) {
   a.max_bps = (int)c.max_bps;
   a.tiles = (int)p.tiles;
   a.tiles_max = (int)p.tiles_max;
-  a.items = (int)p.items;
   a.room = (int)p.room;
+  if (p.list) {   // (the workspace is sized for either kind of pool)
+    const int64_t room = rows_room(c.head_dim, c.num_kv_heads, c.k_scale != nullptr);
+    a.room = (int)(room < p.room ? room : p.room);
+  }
+  a.room1 = (int)((device_cus() + c.num_kv_heads - 1) / c.num_kv_heads);
   a.list = p.list;
+  a.cost_shift = p.cost_shift;
   a.unit_splits = (int)p.unit_splits;
   a.subs = (int)subs_of(a.group);
   a.sub_heads = (a.group + a.subs - 1) / a.subs;
@@ -633,10 +459,7 @@ extern "C" int npd_paged_attention_scored(
   hipStream_t st = as_stream(stream);
   if (dtype == NPD_DTYPE_BF16) launch_stream<BF16>(a, st);
   else launch_stream<F16>(a, st);
-  if (p.unit_slots) {
-    if (dtype == NPD_DTYPE_BF16) launch_merge<BF16>(a, st);
-    else launch_merge<F16>(a, st);
-  }
+  if (p.unit_slots) launch_merge(a, dtype, st);
   return check_launch(c.name);
 }
 
@@ -684,18 +507,13 @@ extern "C" int npd_paged_attention_shared(
   a.shared_lens = shared_lens;
   a.num_groups = (int)num_groups;
   a.max_shared = (int)(max_shared_len < max_keys ? max_shared_len : max_keys);
-  if (!grid_ok(num_seqs * num_kv_heads * a.subs * p.unit_splits) ||
-      !grid_ok(p.items * num_kv_heads))
+  if (!grid_ok(num_seqs * num_kv_heads * a.subs * p.unit_splits + (int64_t)a.room * num_kv_heads))
     return fail(NPD_E_INVALID, "%s: too many work items", c.name);
   hipStream_t st = as_stream(stream);
-  launch_rows_any(a, dtype, st);
-  if (dtype == NPD_DTYPE_BF16) {
-    launch_stream<BF16>(a, st);
-    launch_merge<BF16>(a, st);
-  } else {
-    launch_stream<F16>(a, st);
-    launch_merge<F16>(a, st);
-  }
+  if (head_dim <= 64) launch_rows<64>(a, dtype, st);
+  else if (head_dim <= 128) launch_rows<128>(a, dtype, st);
+  else launch_rows<256>(a, dtype, st);
+  launch_merge(a, dtype, st);
   return check_launch(c.name);
 }
 
@@ -739,13 +557,12 @@ extern "C" int npd_paged_prefill_scored(
   a.cu_seqlens_q = cu_seqlens_q;
   a.first_keys = first_keys;
   a.prefix_lens = prefix_lens;
-  if (!grid_ok(p.items * num_kv_heads))
+  if (!grid_ok((int64_t)a.room * num_kv_heads))
     return fail(NPD_E_INVALID, "%s: too many work items", c.name);
   hipStream_t st = as_stream(stream);
-  launch_rows_any(a, dtype, st);
-  if (p.tile_slots) {
-    if (dtype == NPD_DTYPE_BF16) launch_merge<BF16>(a, st);
-    else launch_merge<F16>(a, st);
-  }
+  if (head_dim <= 64) launch_rows<64>(a, dtype, st);
+  else if (head_dim <= 128) launch_rows<128>(a, dtype, st);
+  else launch_rows<256>(a, dtype, st);
+  if (p.tile_slots) launch_merge(a, dtype, st);
   return check_launch(c.name);
 }

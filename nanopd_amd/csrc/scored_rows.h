@@ -25,19 +25,20 @@
 // finite is computed again, key by key over what it sees (redo_row); a finite
 // result had no such product.
 //
-// Parts: a launch that does not fill the chip several times over cuts its tiles
-// into parts of about equal steps (rows_list), from the lengths on the device.
+// Shares: where whole tiles would leave the chip uneven, its workgroups take equal
+// shares of all tiles' steps, laid end to end (rows_share), from the lengths on the
+// device. A share may end one tile, hold whole ones and begin another; the pieces
+// of a tile meet in the merge kernel.
 #pragma once
 
-#include "scored.h"
+#include "scored_stream.h"
 
 namespace npd {
 namespace scored {
 
 constexpr int kThreads = 256;
 constexpr int kListEntries = 512;    // pool blocks listed in LDS at a time
-constexpr int kMinPartSteps = 8;     // shortest part of a tile
-constexpr int kListSlots = kListTiles / 64;
+constexpr int kPieces = 4;           // pieces of a share listed at a time
 
 // LDS position of 16-byte chunk c of tile row r is c ^ swz(r): rows are D * 2
 // bytes apart without padding (direct loads write 1 KB runs), and the swizzle
@@ -82,165 +83,166 @@ struct Bound<F16> {
 
 __device__ __forceinline__ int wave_min_i(int x) { return -wave_max_i(-x); }
 
-// The item of a workgroup: a tile of rows and part `part` of `cut`.
-struct Item {
-  int s;         // block table row
-  int row0;      // first token row of q / out
-  int tokens;    // tokens of the chunk, or sequences of the group
-  int t;         // tile of them
-  int limit;     // keys at or past it belong to no row here (context, or shared keys)
-  int tile;      // index of the tile among all
-  int part, cut;
+// A piece of a workgroup's work: cost units from / est .. to / est of a tile.
+struct Piece {
+  int s;          // block table row
+  int row0;       // first token row of q / out
+  int tokens;     // tokens of the chunk, or sequences of the group
+  int t;          // tile of them
+  int limit;      // keys at or past it belong to no row here (context, or shared keys)
+  int tile;       // index of the tile among all
+  int from, to, est;
 };
 
-// x / d for 0 <= x < 2^21, 0 < d: the fp32 estimate is off by at most one.
-__device__ __forceinline__ int small_div(int x, int d) {
-  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
-  const int r = x - q * d;
-  return q + (r >= d ? 1 : 0) - (r < 0 ? 1 : 0);
-}
-
-// The steps of a part so that all parts fit `room` at once: the mean load, and
-// more while the parts' round-ups pass the room (not where whole tiles do).
-// count(target) gives the parts of all tiles.
-template <class F>
-__device__ __forceinline__ int part_steps(int64_t total, int tiles, int room, F count) {
-  int target = (int)((total + room - 1) / room);
-  target = target < kMinPartSteps ? kMinPartSteps : target;
-  if (tiles < room)
-    for (int k = 0; k < 12 && count(target) > room; ++k) target += 1 + target / 16;
-  return target;
-}
-
-// Item `id` of a kv head, by one wave: the tiles' parts one after another. Chunks:
-// the last tiles first; a tile's steps are those of its causal range and window.
-// Groups: every tile of a group has the steps of its shared keys. false: none.
-__device__ __forceinline__ bool rows_list(const Args& a, int id, int lane, Item& it) {
-  const int G = a.group, cap = a.max_bps * a.block_size;
-  if (!a.cu_seqlens_q) {
-    int64_t total = 0;
-    int tiles = 0;
-    auto at = [&](int g, Group& r, int& nt, int& n) {
-      r = Group{0, 0, 0, 0};
-      nt = n = 0;
-      if (g < a.num_groups) {
-        r = group_at(a, g);
-        nt = (r.seqs * G + kTileRows - 1) / kTileRows;
-        n = (r.shared + kStepKeys - 1) / kStepKeys;
-      }
-    };
-    Group r;
-    int nt, n;
-    for (int g0 = 0; g0 < a.num_groups; g0 += 64) {
-      at(g0 + lane, r, nt, n);
-      // in pieces of 2^15 steps, so that the wave sums stay in 31 bits
-      const int sum = wave_sum_i(nt * (n >> 6)), low = wave_sum_i(nt * (n & 63));
-      total += (int64_t)sum * 64 + low;
-      tiles += wave_sum_i(n > 0 ? nt : 0);
-    }
-    auto parts = [](int nn, int target) { return (nn + target - 1) / target; };
-    const int target = part_steps(total, tiles, a.room, [&](int tg) {
-      int c = 0;
-      for (int g0 = 0; g0 < a.num_groups; g0 += 64) {
-        if (a.num_groups > 64) at(g0 + lane, r, nt, n);
-        c += wave_sum_i(nt * parts(n, tg));
-      }
-      return c;
-    });
-    int base = 0, tbase = 0;
-    for (int g0 = 0; g0 < a.num_groups; g0 += 64) {
-      if (a.num_groups > 64) at(g0 + lane, r, nt, n);
-      const int cut = parts(n, target);
-      const int ic = wave_scan_i(nt * cut), tc = wave_scan_i(nt);
-      const int i0 = base + ic - nt * cut;
-      const uint64_t m = __ballot(id >= i0 && id < base + ic);
-      if (m != 0) {
-        const int sel = __builtin_ctzll(m);
-        auto of = [&](int x) { return __builtin_amdgcn_readlane(x, sel); };
-        it.cut = of(cut);
-        const int e = id - of(i0);
-        it.t = e / it.cut;
-        it.part = e - it.t * it.cut;
-        it.s = it.row0 = of(r.seq0);
-        it.tokens = of(r.seqs);
-        it.limit = of(r.shared);
-        it.tile = tbase + of(tc) - of(nt) + it.t;
-        if (it.tile >= a.tiles) it.cut = 0;   // groups that overlap
-        return true;
-      }
-      base += __builtin_amdgcn_readlane(ic, 63);
-      tbase += __builtin_amdgcn_readlane(tc, 63);
-    }
-    return false;
-  }
-  // chunks: slot (k, lane) is tile i = last - (64 k + lane) of num_seqs * tiles_max
-  const int all = a.num_seqs * a.tiles_max;
+// Pieces from cost `done` on of the share of workgroup id, up to kPieces, by one
+// wave into out (past the share's end: est == 0). The tiles,
+// each at its cost, are laid end to end (chunks: from the last of the last
+// sequence; a tile's steps are those of its causal range, window and first
+// document, an estimate: what its rows see decides) and cut at multiples of the
+// share; a cut near a tile's edge moves there. sum: running costs (kListEntries).
+__device__ __forceinline__ void rows_share(const Args& a, int id, int done, int lane, int* sum, Piece* out) {
+  const int G = a.group, cap = a.max_bps * a.block_size, shift = a.cost_shift;
+  const bool chunks = a.cu_seqlens_q != nullptr;
+  auto cost = [&](int steps) { return max(1, (steps + kTileCost) >> shift); };
   auto chunk = [&](int sq, int& q0, int& ql, int& cx) {
     q0 = clampi(a.cu_seqlens_q[sq], 0, a.total_q);
     ql = clampi(a.cu_seqlens_q[sq + 1], q0, a.total_q) - q0;
     cx = clampi(a.seq_lens[sq], 0, cap);
   };
-  int n[kListSlots];
-  int total = 0, tiles = 0;
-#pragma unroll
-  for (int k = 0; k < kListSlots; ++k) {
-    n[k] = 0;
-    const int i = all - 1 - (64 * k + lane);
-    if (64 * k < all && i >= 0) {
-      const int sq = small_div(i, a.tiles_max), t = i - sq * a.tiles_max;
-      int q0, ql, cx;
-      chunk(sq, q0, ql, cx);
-      if (t * kTileRows < ql * G) {
-        const int p0 = cx - ql + small_div(t * kTileRows, G);
-        const int p1 = cx - ql + min(ql, small_div((t + 1) * kTileRows + G - 1, G));
-        const int lo = a.window > 0 && p0 - a.window + 1 > 0 ? p0 - a.window + 1 : 0;
-        n[k] = max(1, (max(p1, 0) + kStepKeys - 1) / kStepKeys - lo / kStepKeys);
-      }
-    }
-    total += n[k];
-    tiles += n[k] > 0 ? 1 : 0;
-  }
-  total = wave_sum_i(total);
-  tiles = wave_sum_i(tiles);
-  auto parts = [&](int k, int tg) { return small_div(n[k] + tg - 1, tg); };
-  const int target = part_steps(total, tiles, a.room, [&](int tg) {
+  auto group_tiles = [&](const Group& g) { return (int)(((int64_t)g.seqs * G + kTileRows - 1) / kTileRows); };
+  auto group_cost = [&](const Group& g) { return g.shared > 0 ? cost((g.shared + kStepKeys - 1) / kStepKeys) : 0; };
+  // entry e: tile all - 1 - e of num_seqs * tiles_max, or `per` groups
+  const int all = a.num_seqs * a.tiles_max;
+  const int per = chunks ? 1 : (a.num_groups + kListEntries - 1) / kListEntries;
+  const int n = chunks ? all : (a.num_groups + per - 1) / per;
+  int total = 0;
+#pragma unroll 1
+  for (int e0 = 0; e0 < n; e0 += 64) {
+    const int e = e0 + lane;
     int c = 0;
-#pragma unroll
-    for (int k = 0; k < kListSlots; ++k)
-      if (64 * k < all) c += parts(k, tg);
-    return wave_sum_i(c);
-  });
-  int base = 0, i = -1;
-#pragma unroll
-  for (int k = 0; k < kListSlots; ++k)
-    if (64 * k < all && i < 0) {
-      const int cut = parts(k, target);
-      const int ic = wave_scan_i(cut);
-      const uint64_t m = __ballot(id >= base + ic - cut && id < base + ic);
-      if (m != 0) {
-        const int sel = __builtin_ctzll(m);
-        it.cut = __builtin_amdgcn_readlane(cut, sel);
-        it.part = id - (base + __builtin_amdgcn_readlane(ic, sel) - it.cut);
-        i = all - 1 - (64 * k + sel);
+    if (e < n) {
+      if (chunks) {
+        const int i = all - 1 - e, sq = i / a.tiles_max, t = i - sq * a.tiles_max;
+        int q0, ql, cx;
+        chunk(sq, q0, ql, cx);
+        if (t * kTileRows < ql * G) {
+          const int tok = t * kTileRows / G;
+          const int p0 = cx - ql + tok, p1 = cx - ql + min(ql, ((t + 1) * kTileRows + G - 1) / G);
+          int lo = a.first_keys ? a.first_keys[q0 + tok] : 0;
+          if (a.window > 0) lo = max(lo, p0 - a.window + 1);
+          c = cost(max(0, (max(p1, 0) + kStepKeys - 1) / kStepKeys - max(lo, 0) / kStepKeys));
+        }
+      } else {
+#pragma unroll 1
+        for (int g = e * per; g < min((e + 1) * per, a.num_groups); ++g) {
+          const Group r = group_at(a, g);
+          c += group_tiles(r) * group_cost(r);
+        }
       }
-      base += __builtin_amdgcn_readlane(ic, 63);
     }
-  if (i < 0) return false;
-  it.s = i / a.tiles_max;
-  it.t = i - it.s * a.tiles_max;
-  chunk(it.s, it.row0, it.tokens, it.limit);
-  it.tile = (int)((int64_t)it.row0 * G / kTileRows) + it.s + it.t;
-  return true;
+    c = total + wave_scan_i(c);
+    sum[e] = c;
+    total = __builtin_amdgcn_readlane(c, 63);
+  }
+  wave_sync();
+  // cut k of `shares`, at k / shares of the total but for the tilt: the workgroups
+  // of a compute unit do not run equally fast, its waves issue in the order of
+  // their age (three of them: steps of 1.45, 1.9 and 2.45 us; shares that are all
+  // alike end at 64, 81 and 93 us, tilted ones together)
+  // (shares in whole rounds over the compute units, where they are more than one)
+  int shares = min(a.room, total / kMinShare + 1);
+  if (shares > a.room1) shares -= shares % a.room1;
+  const int tilt = clampi(3 * (shares - a.room1) / a.room1, 0, 6);   // sixteenths
+  Piece pc{};
+  // the tile at cost x: its number in its entry, where it begins, its cost
+  int at, own;
+  auto find = [&](int x) {
+    int e = 0;
+#pragma unroll 1
+    for (int e0 = 0; e0 < n; e0 += 64) {
+      const uint64_t m = __ballot(e0 + lane < n && sum[e0 + lane] > x);
+      if (m != 0) {
+        e = e0 + __builtin_ctzll(m);
+        break;
+      }
+    }
+    at = e > 0 ? sum[e - 1] : 0;
+    own = sum[e] - at;
+    if (chunks) {
+      const int i = all - 1 - e;
+      pc.s = i / a.tiles_max;
+      pc.t = i - pc.s * a.tiles_max;
+    } else {
+      Group r = group_at(a, e * per);
+#pragma unroll 1
+      for (int g = e * per + 1; g < min((e + 1) * per, a.num_groups); ++g) {
+        const int c = group_tiles(r) * group_cost(r);
+        if (x < at + c) break;
+        at += c;
+        r = group_at(a, g);
+      }
+      own = max(1, group_cost(r));
+      pc.t = (x - at) / own;
+      at += pc.t * own;
+      pc.s = pc.row0 = r.seq0;
+      pc.tokens = r.seqs;
+      pc.limit = r.shared;
+    }
+  };
+  // a cut between shares
+  auto edge = [&](int k) {
+    if (k >= shares) return total;
+    const int u = (int)((int64_t)total * k / shares);
+    const int x = u + (int)((int64_t)u * (shares - k) / shares * tilt / 16);
+    find(x);
+    return x - at < kNearEdge ? at : at + own - x < kNearEdge ? at + own : x;
+  };
+  int g = edge(id) + done;
+  const int g1 = edge(id + 1);
+#pragma unroll 1
+  for (int p = 0; p < kPieces; ++p) {
+    pc = Piece{};
+    if (g < g1) {
+      find(g);
+      bool ok = true;
+      if (chunks) {
+        chunk(pc.s, pc.row0, pc.tokens, pc.limit);
+        pc.tile = (int)((int64_t)pc.row0 * G / kTileRows) + pc.s + pc.t;
+      } else {
+        Group r;
+        ok = find_group(a, pc.s, lane, r) && r.tile0 + pc.t < a.tiles;   // (not: groups that overlap)
+        pc.tile = r.tile0 + pc.t;
+      }
+      pc.from = g - at;
+      pc.to = min(g1 - at, own);
+      g += pc.to - pc.from;
+      // (not: costs past 2^31, of lists that do not ascend)
+      if (ok && pc.t >= 0 && pc.from >= 0 && pc.to > pc.from) pc.est = own;
+      else g = g1;
+    }
+    if (lane == 0) out[p] = pc;
+  }
 }
 
 // kCapped: no cap, a plain one, or one past kCapPlain.
 enum Capped { kNoCap, kPlainCap, kWideCap };
+template <int D>
+struct RowsLds {
+  static constexpr int kBufs = D > 128 ? 2 : 3;    // K and V tiles
+  char k[kBufs * kStepKeys * D * 2];
+  char v[kBufs * kStepKeys * D * 2];
+  Keys see[kTileRows];        // keys of the rows (read where a step masks)
+  int row[kListEntries];      // pool rows of the segment's blocks
+  int red[4][4];
+  Piece piece[kPieces];
+};
+// One piece of workgroup id of kv head kh.
 template <class TT, int D, bool kF8, Capped kCapped, bool kBias>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(rows_per_cu(D), rows_per_cu(D))))
-void rows_kernel(Args a) {
+__device__ __forceinline__ void rows_piece(const Args& a, const Piece& it, int id, int kh, bool first,
+                                           int tid, RowsLds<D>& lds) {
   constexpr int KT = kStepKeys;
   constexpr int TR = kTileRows;
-  constexpr int kBufs = D > 128 ? 2 : 3;    // K and V tiles in LDS
+  constexpr int kBufs = RowsLds<D>::kBufs;
   constexpr int kAhead = D > 128 ? 4 : 2;   // LDS operand reads ahead of their MFMA
   constexpr int RB = 2 * D;                 // bytes of a tile row
   constexpr int TB = KT * RB;               // bytes of a tile
@@ -249,44 +251,18 @@ void rows_kernel(Args a) {
   constexpr int EB = kF8 ? 1 : 2;
   constexpr bool kCap = kCapped != kNoCap;
   static_assert(KT == 32 && NI >= 1, "one 32-key block per step");
-  __shared__ __attribute__((aligned(1024))) char s_k[kBufs * TB];
-  __shared__ __attribute__((aligned(1024))) char s_v[kBufs * TB];
-  __shared__ int s_row[kListEntries];
-  __shared__ int s_red[4][4];
-  __shared__ Keys s_see[TR];   // keys of the rows (read where a step masks)
-  __shared__ Item s_item;
-  const int tid = threadIdx.x, lane = tid & 63;
+  char* s_k = lds.k;
+  char* s_v = lds.v;
+  int* s_row = lds.row;
+  auto& s_red = lds.red;
+  Keys* s_see = lds.see;
+  const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hf = lane >> 5, c32 = lane & 31;
   const int G = a.group, d = a.head_dim, bs = a.block_size;
   const int cap_keys = a.max_bps * bs;
   auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
-  // ---- the item: kv head fastest (with 8 of them each XCD's L2 serves one)
-  const int kh = (int)blockIdx.x % a.num_kv_heads, id = (int)blockIdx.x / a.num_kv_heads;
-  Item it;
-  if (a.list) {
-    if (wave == 0) {
-      Item w{};
-      rows_list(a, id, lane, w);    // cut 0: no item
-      if (lane == 0) s_item = w;
-    }
-    __syncthreads();
-    it = Item{uni(s_item.s), uni(s_item.row0), uni(s_item.tokens), uni(s_item.t),
-              uni(s_item.limit), uni(s_item.tile), uni(s_item.part), uni(s_item.cut)};
-    if (it.cut == 0) return;
-  } else {
-    // whole tiles of chunks, the last of a sequence first (it sees the most keys)
-    it.s = id / a.tiles_max;
-    it.t = a.tiles_max - 1 - (id - it.s * a.tiles_max);
-    it.row0 = clampi(a.cu_seqlens_q[it.s], 0, a.total_q);
-    it.tokens = clampi(a.cu_seqlens_q[it.s + 1], it.row0, a.total_q) - it.row0;
-    it.limit = clampi(a.seq_lens[it.s], 0, cap_keys);
-    it.part = 0;
-    it.cut = 1;
-    it.tile = 0;
-    if ((int64_t)it.t * TR >= (int64_t)it.tokens * G) return;
-  }
   const int frows = it.tokens * G;
 
   // ---- this lane's row (past the last: a copy of it, not stored)
@@ -306,16 +282,28 @@ void rows_kernel(Args a) {
     return r;
   };
   const Row row = row_of(c32);
+  const int row_len = a.cu_seqlens_q ? 0 : a.seq_lens[row.q];
+  const int row_first = a.first_keys ? a.first_keys[row.q] : 0;
+  const int row_pre = a.prefix_lens ? a.prefix_lens[it.s] : 0;
+
+  // ---- queries as B operands: qb[c] = Q[row][16c + 8 hf ..], zeros past the row
+  u32x4 qb[NC];
+  {
+    const uint16_t* qp = a.q + row.strides(a.q_stride_token, a.q_stride_head);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      qb[c] = c * 16 + hf * 8 < d ? *reinterpret_cast<const u32x4*>(qp + c * 16 + hf * 8)
+                                  : u32x4{0, 0, 0, 0};
+  }
   int pos, ctx;
   if (a.cu_seqlens_q) {
     ctx = it.limit;
     pos = ctx - it.tokens + row.tok;
   } else {
-    ctx = clampi(a.seq_lens[row.q], 0, cap_keys);
+    ctx = clampi(row_len, 0, cap_keys);
     pos = ctx - 1;
   }
-  Keys see = row_keys(pos, ctx, a.first_keys ? a.first_keys[row.q] : 0,
-                      a.prefix_lens ? a.prefix_lens[it.s] : 0, a.window);
+  Keys see = row_keys(pos, ctx, row_first, row_pre, a.window);
   see.hi = min(see.hi, it.limit);
   see.pre = min(see.pre, it.limit);
   if (see.lo >= see.hi) see.lo = see.hi = 0;          // empty ranges are [0, 0)
@@ -357,23 +345,22 @@ void rows_kernel(Args a) {
     fs0 = fs1 = 0;
   }
   const int nfar = fs1 - fs0, nsteps = nfar + ns1 - ns0;
-  const bool merged = a.cu_groups || it.cut > 1;
-  if (a.list && it.part == 0 && tid == 0) {
-    a.tile_items[2 * (it.tile * a.num_kv_heads + kh)] = id;
-    a.tile_items[2 * (it.tile * a.num_kv_heads + kh) + 1] = it.cut;
+  // steps of the piece; where its results go: rows of out, or a slot of partials
+  // (a share's first piece may begin within a tile, its last end within one)
+  const bool whole_tile = it.from == 0 && it.to == it.est;
+  const bool merged = a.cu_groups || !whole_tile;
+  const int64_t slot = whole_tile ? 2 * (int64_t)a.room + it.tile : 2 * (int64_t)id + (first ? 0 : 1);
+  if (tid == 0 && a.tile_items) {
+    int32_t* e = a.tile_items + 4 * ((int64_t)it.tile * a.num_kv_heads + kh);
+    if (it.from == 0) {
+      e[0] = (int)slot;
+      e[1] = id;
+    }
+    if (it.to == it.est) e[2] = id;
   }
-  const int base = nsteps / it.cut, rem = nsteps - base * it.cut;
-  const int st0 = it.part * base + min(it.part, rem), st1 = st0 + base + (it.part < rem ? 1 : 0);
+  const int st0 = (int)((int64_t)it.from * nsteps / it.est);
+  const int st1 = (int)((int64_t)it.to * nsteps / it.est);
 
-  // ---- queries as B operands: qb[c] = Q[row][16c + 8 hf ..], zeros past the row
-  u32x4 qb[NC];
-  {
-    const uint16_t* qp = a.q + row.strides(a.q_stride_token, a.q_stride_head);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-      qb[c] = c * 16 + hf * 8 < d ? *reinterpret_cast<const u32x4*>(qp + c * 16 + hf * 8)
-                                  : u32x4{0, 0, 0, 0};
-  }
   const float kscale = kF8 ? a.k_scale[kh] : 1.f;
   const float c2 = a.scale_log2 * kscale, cin = a.cap_in * kscale, capA = a.cap_log2;
   const float slope = kBias ? a.slopes[row.h] * kLog2e : 0.f;
@@ -691,7 +678,7 @@ void rows_kernel(Args a) {
   const uint64_t bad = __ballot(!(chk < INFINITY));   // an infinity or NaN among the row's sums
   const uint32_t bad_rows = (uint32_t)bad | (uint32_t)(bad >> 32);
   const float oscale = kF8 ? a.v_scale[kh] : 1.f;
-  const int64_t slot0 = (int64_t)blockIdx.x * TR + wave * 32;
+  const int64_t slot0 = (slot * a.num_kv_heads + kh) * TR + wave * 32;
   int c = c32;   // (opaque: the row is found again, not kept through the loop)
   asm volatile("" : "+v"(c));
   const Row dst = row_of(c);
@@ -774,29 +761,106 @@ void rows_kernel(Args a) {
         *reinterpret_cast<u32x2*>(a.out + rr.strides(a.out_stride_token, a.out_stride_head) + d0) =
             u32x2{TT::pack2(o[0] * inv, o[1] * inv), TT::pack2(o[2] * inv, o[3] * inv)};
     } else {
-      const int64_t slot = slot0 + w;
-      if (on) *reinterpret_cast<f32x4*>(a.tile_o + slot * d + d0) = f32x4{o[0], o[1], o[2], o[3]};
+      if (on) *reinterpret_cast<f32x4*>(a.tile_o + (slot0 + w) * d + d0) = f32x4{o[0], o[1], o[2], o[3]};
       if (lane == 0) {
-        a.tile_ml[slot * 2] = m;
-        a.tile_ml[slot * 2 + 1] = l;
+        a.tile_ml[(slot0 + w) * 2] = m;
+        a.tile_ml[(slot0 + w) * 2 + 1] = l;
       }
     }
   }
 }
 
+// All pieces of workgroup `block` (kv head fastest: with 8 of them each XCD's L2
+// serves one). Each piece takes the arguments and its thread number afresh, so
+// that nothing derived from them stays in registers from piece to piece.
+template <class TT, int D, bool kF8, Capped kCapped, bool kBias>
+__device__ __forceinline__ void rows_group(int block, RowsLds<D>& lds) {
+  typedef const Args __attribute__((address_space(4))) KernArgs;
+  auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  for (int done = 0, n = 0;; ++n) {
+    KernArgs* ka = (KernArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    int tid = threadIdx.x;
+    asm volatile("" : "+s"(ka), "+v"(tid));
+    const Args& a = *(const Args*)ka;
+    const int id = block / a.num_kv_heads, kh = block - id * a.num_kv_heads;
+    Piece it;
+    if (a.list) {
+      __syncthreads();   // the last piece's reads are done
+      if (n % kPieces == 0) {
+        if (uni(tid >> 6) == 0) rows_share(a, id, done, tid & 63, lds.row, lds.piece);
+        __syncthreads();
+      }
+      const Piece& p = lds.piece[n % kPieces];
+      it = Piece{uni(p.s), uni(p.row0), uni(p.tokens), uni(p.t), uni(p.limit), uni(p.tile),
+                 uni(p.from), uni(p.to), uni(p.est)};
+      if (it.est == 0) return;
+    } else {
+      // whole tiles of chunks, the last of a sequence first (it sees the most keys)
+      it.s = id / a.tiles_max;
+      it.t = a.tiles_max - 1 - (id - it.s * a.tiles_max);
+      it.row0 = clampi(a.cu_seqlens_q[it.s], 0, a.total_q);
+      it.tokens = clampi(a.cu_seqlens_q[it.s + 1], it.row0, a.total_q) - it.row0;
+      it.limit = clampi(a.seq_lens[it.s], 0, a.max_bps * a.block_size);
+      it.tile = it.from = 0;
+      it.to = it.est = 1;
+      if ((int64_t)it.t * kTileRows >= (int64_t)it.tokens * a.group) return;
+    }
+    rows_piece<TT, D, kF8, kCapped, kBias>(a, it, id, kh, n == 0, tid, lds);
+    if (!a.list) return;
+    done += it.to - it.from;
+  }
+}
+
+template <class TT, int D, bool kF8, Capped kCapped, bool kBias>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(rows_per_cu(D, kF8), rows_per_cu(D, kF8))))
+void chunks_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) RowsLds<D> lds;
+  rows_group<TT, D, kF8, kCapped, kBias>(blockIdx.x, lds);
+}
+
+// Groups: workgroups for the shared keys, then four stream units each for the
+// sequences' own keys: the one kind waits on the matrix cores, the other on HBM.
+template <class TT, int D, bool kF8, Capped kCapped, bool kBias>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(rows_per_cu(D, kF8), rows_per_cu(D, kF8))))
+void shared_kernel(Args a) {
+  union Lds {
+    RowsLds<D> rows;
+    StreamLds<D> stream[kThreads / 64];
+  };
+  __shared__ __attribute__((aligned(1024))) Lds lds;
+  const int n = a.room * a.num_kv_heads;
+  if ((int)blockIdx.x < n) {
+    rows_group<TT, D, kF8, kCapped, kBias>(blockIdx.x, lds.rows);
+  } else {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    stream_unit<TT, D, kF8>(a, ((int)blockIdx.x - n) * (kThreads / 64) + wave, threadIdx.x & 63,
+                            lds.stream[wave]);
+  }
+}
+
+template <class TT, int D, bool kF8, Capped kCapped, bool kBias>
+void launch_rows_k(const Args& a, hipStream_t st) {
+  int64_t n = (int64_t)a.room * a.num_kv_heads;
+  if (a.cu_seqlens_q) {
+    hipLaunchKernelGGL((chunks_kernel<TT, D, kF8, kCapped, kBias>), dim3((unsigned)n), dim3(kThreads), 0, st, a);
+  } else {
+    const int64_t units = (int64_t)a.num_seqs * a.num_kv_heads * a.subs * a.unit_splits;
+    n += (units + kThreads / 64 - 1) / (kThreads / 64);
+    hipLaunchKernelGGL((shared_kernel<TT, D, kF8, kCapped, kBias>), dim3((unsigned)n), dim3(kThreads), 0, st, a);
+  }
+}
 template <class TT, int D, bool kF8>
 void launch_rows_f(const Args& a, hipStream_t st) {
-  const dim3 g((unsigned)(a.items * a.num_kv_heads)), b(kThreads);
   const bool bias = a.slopes != nullptr;
   if (a.cap_log2 <= 0.f) {
-    if (bias) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kNoCap, true>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kNoCap, false>), g, b, 0, st, a);
+    if (bias) launch_rows_k<TT, D, kF8, kNoCap, true>(a, st);
+    else launch_rows_k<TT, D, kF8, kNoCap, false>(a, st);
   } else if (a.cap_wide) {
-    if (bias) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kWideCap, true>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kWideCap, false>), g, b, 0, st, a);
+    if (bias) launch_rows_k<TT, D, kF8, kWideCap, true>(a, st);
+    else launch_rows_k<TT, D, kF8, kWideCap, false>(a, st);
   } else {
-    if (bias) hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kPlainCap, true>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((rows_kernel<TT, D, kF8, kPlainCap, false>), g, b, 0, st, a);
+    if (bias) launch_rows_k<TT, D, kF8, kPlainCap, true>(a, st);
+    else launch_rows_k<TT, D, kF8, kPlainCap, false>(a, st);
   }
 }
 
