@@ -248,7 +248,8 @@ void plan_list(Plan& p, int64_t tiles, int64_t steps) {
   const int64_t total = tiles * (steps + kTileCost), most = (total + kMinShare - 1) / kMinShare;
   p.list = true;
   p.room = p.room < most ? p.room : most < 1 ? 1 : most;
-  while (((steps + kTileCost) >> p.cost_shift) + 1 > (INT32_MAX / 2) / tiles) ++p.cost_shift;
+  while (p.cost_shift < 30 && ((steps + kTileCost) >> p.cost_shift) + 1 > (INT32_MAX / 2) / tiles)
+    ++p.cost_shift;
 }
 Plan shared_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                  int64_t max_keys, int64_t num_groups, int64_t max_shared) {
@@ -507,7 +508,7 @@ extern "C" int npd_paged_attention_shared(
   a.shared_lens = shared_lens;
   a.num_groups = (int)num_groups;
   a.max_shared = (int)(max_shared_len < max_keys ? max_shared_len : max_keys);
-  if (!grid_ok(num_seqs * num_kv_heads * a.subs * p.unit_splits + (int64_t)a.room * num_kv_heads))
+  if (!grid_ok(num_seqs * num_kv_heads * a.subs * p.unit_splits + p.room * num_kv_heads))
     return fail(NPD_E_INVALID, "%s: too many work items", c.name);
   hipStream_t st = as_stream(stream);
   if (head_dim <= 64) launch_rows<64>(a, dtype, st);
@@ -557,7 +558,7 @@ extern "C" int npd_paged_prefill_scored(
   a.cu_seqlens_q = cu_seqlens_q;
   a.first_keys = first_keys;
   a.prefix_lens = prefix_lens;
-  if (!grid_ok((int64_t)a.room * num_kv_heads))
+  if (!grid_ok(p.room * num_kv_heads))
     return fail(NPD_E_INVALID, "%s: too many work items", c.name);
   hipStream_t st = as_stream(stream);
   if (head_dim <= 64) launch_rows<64>(a, dtype, st);

@@ -39,6 +39,7 @@ __all__ = [
     "paged_prefill_attention", "copy_blocks", "pack_metadata", "BatchMetadata",
     "attention_workspace_bytes", "prefill_workspace_bytes", "qk_norm_rope_store",
     "paged_attention_scored", "paged_prefill_attention_scored", "paged_attention_shared",
+    "SharedPrefixes", "find_shared_prefixes",
     "scored_workspace_bytes", "prefill_scored_workspace_bytes", "shared_workspace_bytes",
     "block_norms",
 ]
@@ -924,6 +925,41 @@ def paged_attention_shared(out: torch.Tensor, query: torch.Tensor, key_cache: to
              out.stride(0), out.stride(1), ws_ptr, ws_bytes, code)
 
 
+class SharedPrefixes(NamedTuple):
+    """What :func:`paged_attention_shared` takes of a batch's groups."""
+    cu_groups: torch.Tensor     # int32 [num_groups + 1]
+    shared_lens: torch.Tensor   # int32 [num_groups]
+    max_shared_len: int
+
+
+def find_shared_prefixes(tables: Sequence[Sequence[int]], lens: Sequence[int], block_size: int,
+                         device: torch.device | str) -> SharedPrefixes | None:
+    """The groups of a decode batch, from its block tables on the host: runs of
+    neighbouring sequences whose tables begin with the same blocks, as forks of one
+    prompt do (BlockSpaceManager.fork). A group shares the whole blocks that all its
+    tables have in common, of the tokens that its shortest sequence holds; a sequence
+    that would leave it less than half of them begins its own. None: no two
+    neighbours share a block."""
+    cu, shared = [0], []
+    common: list = []
+    for i, (t, n) in enumerate(zip(tables, lens)):
+        full = list(t[: int(n) // block_size])
+        k = 0
+        while k < min(len(common), len(full)) and common[k] == full[k]:
+            k += 1
+        if k > 0 and (shared[-1] == 0 or 2 * k >= len(common)):
+            common = common[:k]
+            cu[-1], shared[-1] = i + 1, k * block_size
+        else:
+            common = full
+            cu.append(i + 1)
+            shared.append(0)
+    if not any(shared):
+        return None
+    packed = torch.tensor(cu + shared, dtype=torch.int32).to(device)
+    return SharedPrefixes(packed[: len(cu)], packed[len(cu):], max(shared))
+
+
 def paged_prefill_attention_scored(out: torch.Tensor, query: torch.Tensor,
                                    key_cache: torch.Tensor, value_cache: torch.Tensor,
                                    block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -1023,8 +1059,8 @@ def block_norms(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor 
     over the last dim of 2-D tensors. The new x is left in ``x``, or in ``x_out``
     if given (which may be delta). gate broadcasts against x: [width], [rows, 1] or
     [rows, width]. 2-byte CUDA tensors of up to 8192 columns run as one launch with
-    fp32 inside; others, and calls that record a gradient, as torch operations,
-    which take a new x_out only through x (they refuse what does not fit)."""
+    fp32 inside; others, and calls that record a gradient, as torch operations
+    (which refuse what does not fit, or an x that may not be written in place)."""
     ts = [t for t in (delta, post_weight, weight, x_out) if t is not None]
     if (x.dim() == 2 and x.size(1) <= 8192 and delta.shape == x.shape and _rows_16(x, *ts)
             and (post_weight is None or post_weight.shape == x.shape[1:])

@@ -28,6 +28,10 @@ has them (:101-104). Qwen3Config's qk_norm=False, qkv_bias=True and
 tie_word_embeddings=True give that layer (Qwen2: q/k/v biases, no q/k norms,
 tied LM head on the 1.5B model); the fused prologue then runs without norm
 weights.
+Further options, off by default, change the layer itself (the reference has no
+counterpart): attn_softcap caps the attention scores, window limits how far back
+they reach, block_norms also norms what a block returns before it joins the
+residual stream. StepBatch.shared names the prefixes that decode sequences share.
 """
 from __future__ import annotations
 
@@ -56,6 +60,9 @@ class Qwen3Config:
     qk_norm: bool = True              # per-head q/k RMSNorm (Qwen3); False: Qwen2 / Llama
     qkv_bias: bool = False            # q/k/v projection biases (Qwen2)
     tie_word_embeddings: bool = False  # LM head = embedding (Qwen2-1.5B)
+    attn_softcap: float = 0.0         # scores capped as c * tanh(t / c) (0: not)
+    window: int = 0                   # keys that a token sees, itself included (0: all)
+    block_norms: bool = False         # RMSNorm of what attention and MLP return
 
     @property
     def num_params(self) -> int:
@@ -63,7 +70,8 @@ class Qwen3Config:
         qkv = self.hidden * width + (width if self.qkv_bias else 0)
         o = self.num_heads * self.head_dim * self.hidden
         mlp = 3 * self.hidden * self.intermediate
-        norms = 2 * self.hidden + (2 * self.head_dim if self.qk_norm else 0)
+        norms = (4 if self.block_norms else 2) * self.hidden
+        norms += 2 * self.head_dim if self.qk_norm else 0
         heads = (1 if self.tie_word_embeddings else 2) * self.vocab * self.hidden
         return self.num_layers * (qkv + o + mlp + norms) + heads + self.hidden
 
@@ -87,6 +95,7 @@ class StepBatch:
     sample_rows: Optional[torch.Tensor]   # int64 [R]; None: every row
     max_prefill_q: int = 0           # longest prefill chunk (grid bound)
     decode_workspace: Optional[torch.Tensor] = None   # explicit decode-attention workspace
+    shared: Optional[pk.SharedPrefixes] = None   # of the decode sequences (find_shared_prefixes)
 
 
 # attention(layer, q [T,H,D], k_cache, v_cache, batch, out [T,H,D]) -> None
@@ -141,6 +150,8 @@ class PagedQwen3:
                 "k_norm": ones(D) if cfg.qk_norm else None,
                 "o": rnd(E, H * D),
                 "post_norm": ones(E),
+                "attn_out_norm": ones(E) if cfg.block_norms else None,
+                "mlp_out_norm": ones(E) if cfg.block_norms else None,
                 "gate_up": rnd(2 * cfg.intermediate, E),
                 "down": rnd(E, cfg.intermediate),
             })
@@ -206,11 +217,18 @@ class PagedQwen3:
                          b: StepBatch, out: torch.Tensor) -> None:
         m, npf, tp = b.meta, b.num_prefill_seqs, b.num_prefill_tokens
         T = q.size(0)
+        cap, window = self.cfg.attn_softcap, self.cfg.window
+        scored = cap > 0 or window > 0
+        rule = {"softcap": cap, "window": window}
+        if self.fp8:
+            rule.update(k_scale=self.k_scale[layer], v_scale=self.v_scale[layer])
         if npf:
             args = (out[:tp], q[:tp], kc, vc, m.block_tables[:npf], m.cu_seqlens_q[:npf + 1],
                     m.seq_lens[:npf], self.scale, self.block_size, m.max_blocks_per_seq,
                     max(1, b.max_prefill_q))
-            if self.fp8:
+            if scored:
+                pk.paged_prefill_attention_scored(*args, m.max_seq_len, **rule)
+            elif self.fp8:
                 pk.paged_prefill_attention_fp8(*args, self.k_scale[layer], self.v_scale[layer],
                                                m.max_seq_len)
             else:
@@ -218,7 +236,11 @@ class PagedQwen3:
         if T > tp:
             args = (out[tp:], q[tp:], kc, vc, m.block_tables[npf:], m.seq_lens[npf:], self.scale,
                     self.block_size, m.max_blocks_per_seq)
-            if self.fp8:
+            if b.shared is not None:
+                pk.paged_attention_shared(*args, *b.shared, **rule)
+            elif scored:
+                pk.paged_attention_scored(*args, **rule)
+            elif self.fp8:
                 pk.paged_attention_forward_fp8(*args, self.k_scale[layer], self.v_scale[layer],
                                                workspace=b.decode_workspace)
             else:
@@ -247,12 +269,20 @@ class PagedQwen3:
             self.attention(li, q, kc, vc, b, attn)
             # each residual add joins the norm that follows it (x stays the
             # residual stream); the last one has the sampled rows' norm after it
-            h = pk.add_rms_norm(x, attn.view(T, H * D) @ w["o"].t(), w["post_norm"], cfg.rms_eps)
-            down = pk.silu_mul(h @ w["gate_up"].t()) @ w["down"].t()
-            if li + 1 < cfg.num_layers:
-                h = pk.add_rms_norm(x, down, self.layers[li + 1]["in_norm"], cfg.rms_eps)
+            o = attn.view(T, H * D) @ w["o"].t()
+            if cfg.block_norms:
+                h = pk.block_norms(x, o, w["attn_out_norm"], w["post_norm"], cfg.rms_eps)
             else:
+                h = pk.add_rms_norm(x, o, w["post_norm"], cfg.rms_eps)
+            down = pk.silu_mul(h @ w["gate_up"].t()) @ w["down"].t()
+            last = li + 1 == cfg.num_layers
+            next_norm = None if last else self.layers[li + 1]["in_norm"]
+            if cfg.block_norms:
+                h = pk.block_norms(x, down, w["mlp_out_norm"], next_norm, cfg.rms_eps)
+            elif last:
                 x = x + down
+            else:
+                h = pk.add_rms_norm(x, down, next_norm, cfg.rms_eps)
         if b.sample_rows is not None:
             x = x.index_select(0, b.sample_rows)
         xs = F.rms_norm(x, (E,), self.final_norm, cfg.rms_eps)
@@ -271,6 +301,8 @@ class PagedQwen3:
             t = sd[name]
             return t.to(device=self.device, dtype=self.dtype)
 
+        if self.cfg.block_norms:
+            raise ValueError("no Qwen3 or Qwen2 checkpoint has norms after its blocks (block_norms)")
         self.embed.copy_(get("model.embed_tokens.weight"))
         for i, w in enumerate(self.layers):
             p = f"model.layers.{i}."
