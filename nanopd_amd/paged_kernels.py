@@ -720,83 +720,103 @@ def qk_norm_rope_store(q_out: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 # Attention with changed scores
 # ---------------------------------------------------------------------------
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _call_on(device: int, name: str, *args) -> None:
     """The library call with the tensors' device current: kernels launch on the
     stream of the device that is."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, _stream(dev))
+    if device == _get_device() and _raw_stream is not None:
+        _lib.call(name, *args, _raw_stream(device))
     else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, _stream(dev))
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _stream(torch.device("cuda", device)))
 
 
-def _score_rule(what, out, query, key_cache, value_cache, block_tables, scale, block_size,
+def _score_rule(what, out, query, key_cache, value_cache, block_tables, seqs, scale, block_size,
                 max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale, lens):
-    """Checks that the scored ops share. lens: (tensor, name, least length) of the
-    int32 vectors, None where not given. Returns the cache sizes, the element code
-    and the pointers of the score arguments."""
+    """Checks that the scored ops share. seqs: block table rows wanted (None: as many
+    as tokens); lens: (tensor, name, least length) of the int32 vectors (length None:
+    as many as tokens; tensors in _optional may be None). Returns (tokens, heads,
+    device), the cache sizes, the element code, the score arguments, the scale
+    pointers and the strides."""
     if not (isinstance(query, torch.Tensor) and query.is_cuda):
         _fail("query is must be on CUDA")
-    if not (query.dim() == 3):
+    shape = query.shape
+    if len(shape) != 3:
         _fail(f"{what}: query must be [tokens, num_heads, head_size]")
+    n, h, d = shape
+    dev, dtype = query.get_device(), query.dtype
     fp8 = k_scale is not None or v_scale is not None
     if fp8:
         _fp8_cache_checks(key_cache, value_cache, k_scale, v_scale)
+        if k_scale.get_device() != dev or v_scale.get_device() != dev:
+            _fail(f"k_scale and v_scale must be on {query.device}")
     else:
         _cache_checks(key_cache, value_cache)
-    dev = query.device
-    _int32(block_tables, "block_tables")
-    given = [x for x in lens if x[0] is not None]
-    for t, nm, n in given:
+        if key_cache.dtype is not dtype:
+            _fail("query/cache dtype mismatch")
+    for t in (out, key_cache, value_cache):
+        if t.get_device() != dev:
+            _fail(f"tensor on {t.device}, expected {query.device}")
+    for t, nm, least in lens:
+        if t is None and nm in _optional:
+            continue
         _int32(t, nm)
-        if not (t.dim() == 1 and t.numel() >= n and t.is_contiguous()):
-            _fail(f"{nm} must be a contiguous int32 vector of at least {n}")
-    _same_device(dev, out, key_cache, value_cache, block_tables, *(x[0] for x in given))
-    if fp8:
-        _same_device(dev, k_scale, v_scale)
-    h, d = query.size(1), query.size(2)
+        if (t.get_device() != dev or t.dim() != 1 or t.numel() < (n if least is None else least)
+                or not t.is_contiguous()):
+            _fail(f"{nm} must be a contiguous int32 vector of at least {n if least is None else least} "
+                  f"on {query.device}")
     num_blocks, kvh, bs, cd = key_cache.shape
-    if not (cd == d):
+    if cd != d:
         _fail(f"head_dim {d} does not match cache head_dim {cd}")
-    if not (int(block_size) == bs):
+    if int(block_size) != bs:
         _fail(f"block_size {block_size} does not match cache block size {bs}")
     if not (kvh > 0 and h > 0 and h % kvh == 0):
         _fail(f"num_heads {h} is not a multiple of num_kv_heads {kvh}")
-    if not (out.shape == query.shape and out.dtype == query.dtype):
+    if not (out.shape == shape and out.dtype is dtype):
         _fail("out must match query")
-    if not (fp8 or query.dtype == key_cache.dtype):
-        _fail("query/cache dtype mismatch")
-    code = _dtype_code(query, what)
+    code = _DTYPES.get(dtype)
+    if code is None:
+        _dtype_code(query, what)
     mb = int(max_num_blocks_per_seq)
-    if not (block_tables.dim() == 2 and block_tables.size(1) == mb and block_tables.is_contiguous()):
-        _fail("block_tables must be a contiguous [num_seqs, max_num_blocks_per_seq] tensor")
-    if not (query.stride(2) == 1 and out.stride(2) == 1):
+    _int32(block_tables, "block_tables")
+    table = block_tables.shape
+    if (len(table) != 2 or table[0] < (n if seqs is None else seqs) or table[1] != mb
+            or not block_tables.is_contiguous() or block_tables.get_device() != dev):
+        _fail("block_tables must be a contiguous [num_seqs, max_num_blocks_per_seq] tensor on "
+              f"{query.device}")
+    qs, os = query.stride(), out.stride()
+    if not (qs[2] == 1 and os[2] == 1):
         _fail("head_dim must be the contiguous dim")
     slopes = 0
     if alibi_slopes is not None:
-        if not (isinstance(alibi_slopes, torch.Tensor) and alibi_slopes.dtype == torch.float32
-                and alibi_slopes.shape == (h,) and alibi_slopes.is_contiguous()):
-            _fail("alibi_slopes must be a contiguous float32 [num_heads] tensor")
-        _same_device(dev, alibi_slopes)
+        if not (isinstance(alibi_slopes, torch.Tensor) and alibi_slopes.dtype is torch.float32
+                and alibi_slopes.shape == (h,) and alibi_slopes.is_contiguous()
+                and alibi_slopes.get_device() == dev):
+            _fail(f"alibi_slopes must be a contiguous float32 [num_heads] tensor on {query.device}")
         slopes = alibi_slopes.data_ptr()
     rule = (float(scale), float(softcap), slopes, int(window))
     scales = (k_scale.data_ptr(), v_scale.data_ptr()) if fp8 else (0, 0)
-    return (num_blocks, kvh, bs, d, mb), code, rule, scales
+    return (n, h, dev), (num_blocks, kvh, bs, d, mb), code, rule, scales, (qs[0], qs[1], os[0], os[1])
 
 
-def _scored_workspace(workspace, need: int, dev: torch.device):
+_optional = ("first_keys", "prefix_lens")
+
+
+def _scored_workspace(workspace, need: int, device: int):
     """(the workspace, its pointer, its bytes): the caller's, or one of this call
     from torch's allocator, which orders its reuse by stream and leaves it to a
     graph that is being captured."""
     if need <= 0:
         return None, 0, 0
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    else:
-        _same_device(dev, workspace)
-        if not (workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need):
-            _fail(f"workspace of {need} bytes needed")
-    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        return workspace, workspace.data_ptr(), need
+    size = workspace.numel() * workspace.element_size()
+    if not (workspace.get_device() == device and workspace.is_contiguous() and size >= need):
+        _fail(f"workspace of {need} bytes on cuda:{device} needed")
+    return workspace, workspace.data_ptr(), size
 
 
 @functools.lru_cache(maxsize=1024)
@@ -856,26 +876,22 @@ def paged_attention_scored(out: torch.Tensor, query: torch.Tensor, key_cache: to
     group. ``workspace``: at least :func:`scored_workspace_bytes` bytes (its
     contents do not matter) in place of one allocated per call.
     """
-    s = query.size(0) if isinstance(query, torch.Tensor) and query.dim() == 3 else 0
-    (num_blocks, kvh, bs, d, mb), code, rule, scales = _score_rule(
-        "paged_attention_scored", out, query, key_cache, value_cache, block_tables, scale,
+    (s, h, dev), (num_blocks, kvh, bs, d, mb), code, rule, scales, strides = _score_rule(
+        "paged_attention_scored", out, query, key_cache, value_cache, block_tables, None, scale,
         block_size, max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale,
-        ((seq_lens, "seq_lens", s), (first_keys, "first_keys", s), (prefix_lens, "prefix_lens", s)))
-    _int32(seq_lens, "seq_lens")
-    if not (block_tables.size(0) >= s):
-        _fail("block_tables must be [num_seqs, max_num_blocks_per_seq]")
+        ((seq_lens, "seq_lens", None), (first_keys, "first_keys", None),
+         (prefix_lens, "prefix_lens", None)))
     if s == 0:
         return
-    h, dev = query.size(1), query.device
-    need = _scored_ws("npd_paged_attention_scored_workspace_size", s, h, kvh, d, bs, mb, int(window),
-                      int(prefix_lens is not None))
+    need = _scored_ws("npd_paged_attention_scored_workspace_size", s, h, kvh, d, bs, mb, rule[3],
+                      prefix_lens is not None)
     ws, ws_ptr, ws_bytes = _scored_workspace(workspace, need, dev)
     _call_on(dev, "npd_paged_attention_scored", out.data_ptr(), query.data_ptr(),
              key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
              seq_lens.data_ptr(), s, h, kvh, d, num_blocks, bs, mb, *rule,
              0 if first_keys is None else first_keys.data_ptr(),
-             0 if prefix_lens is None else prefix_lens.data_ptr(), *scales, query.stride(0),
-             query.stride(1), out.stride(0), out.stride(1), ws_ptr, ws_bytes, code)
+             0 if prefix_lens is None else prefix_lens.data_ptr(), *scales, *strides, ws_ptr,
+             ws_bytes, code)
 
 
 def paged_attention_shared(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor,
@@ -899,30 +915,24 @@ def paged_attention_shared(out: torch.Tensor, query: torch.Tensor, key_cache: to
     bound on shared_lens (shared keys past it are read per sequence).
     ``workspace``: at least :func:`shared_workspace_bytes` bytes.
     """
-    s = query.size(0) if isinstance(query, torch.Tensor) and query.dim() == 3 else 0
     _int32(cu_groups, "cu_groups")
     ng = cu_groups.numel() - 1
-    if not (cu_groups.dim() == 1 and ng >= 1):
+    if ng < 1:
         _fail("cu_groups must be a contiguous int32 [num_groups + 1] vector of one group at least")
-    (num_blocks, kvh, bs, d, mb), code, rule, scales = _score_rule(
-        "paged_attention_shared", out, query, key_cache, value_cache, block_tables, scale,
+    (s, h, dev), (num_blocks, kvh, bs, d, mb), code, rule, scales, strides = _score_rule(
+        "paged_attention_shared", out, query, key_cache, value_cache, block_tables, None, scale,
         block_size, max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale,
-        ((seq_lens, "seq_lens", s), (cu_groups, "cu_groups", ng + 1), (shared_lens, "shared_lens", ng)))
-    _int32(seq_lens, "seq_lens")
-    _int32(shared_lens, "shared_lens")
-    if not (block_tables.size(0) >= s):
-        _fail("block_tables must be [num_seqs, max_num_blocks_per_seq]")
+        ((seq_lens, "seq_lens", None), (cu_groups, "cu_groups", ng + 1),
+         (shared_lens, "shared_lens", ng)))
     if s == 0:
         return
-    h, dev = query.size(1), query.device
     mshared = min(int(max_shared_len), mb * bs)
     need = _scored_ws("npd_paged_attention_shared_workspace_size", s, h, kvh, d, bs, mb, ng, mshared)
     ws, ws_ptr, ws_bytes = _scored_workspace(workspace, need, dev)
     _call_on(dev, "npd_paged_attention_shared", out.data_ptr(), query.data_ptr(),
              key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
              seq_lens.data_ptr(), cu_groups.data_ptr(), shared_lens.data_ptr(), s, ng, mshared, h,
-             kvh, d, num_blocks, bs, mb, *rule, *scales, query.stride(0), query.stride(1),
-             out.stride(0), out.stride(1), ws_ptr, ws_bytes, code)
+             kvh, d, num_blocks, bs, mb, *rule, *scales, *strides, ws_ptr, ws_bytes, code)
 
 
 class SharedPrefixes(NamedTuple):
@@ -982,22 +992,17 @@ def paged_prefill_attention_scored(out: torch.Tensor, query: torch.Tensor,
     cu_seqlens_q[-1] are left as they were. ``workspace``: at least
     :func:`prefill_scored_workspace_bytes` bytes (contents do not matter).
     """
-    tq = query.size(0) if isinstance(query, torch.Tensor) and query.dim() == 3 else 0
     _int32(cu_seqlens_q, "cu_seqlens_q")
     ns = cu_seqlens_q.numel() - 1
-    if not (cu_seqlens_q.dim() == 1 and ns >= 0):
+    if ns < 0:
         _fail("cu_seqlens_q must be a contiguous [num_seqs + 1] tensor")
-    (num_blocks, kvh, bs, d, mb), code, rule, scales = _score_rule(
-        "paged_prefill_attention_scored", out, query, key_cache, value_cache, block_tables, scale,
-        block_size, max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale,
+    (tq, h, dev), (num_blocks, kvh, bs, d, mb), code, rule, scales, strides = _score_rule(
+        "paged_prefill_attention_scored", out, query, key_cache, value_cache, block_tables, ns,
+        scale, block_size, max_num_blocks_per_seq, softcap, alibi_slopes, window, k_scale, v_scale,
         ((cu_seqlens_q, "cu_seqlens_q", ns + 1), (context_lens, "context_lens", ns),
-         (first_keys, "first_keys", tq), (prefix_lens, "prefix_lens", ns)))
-    _int32(context_lens, "context_lens")
-    if not (block_tables.size(0) >= ns):
-        _fail("block_tables must be [num_seqs, max_num_blocks_per_seq]")
+         (first_keys, "first_keys", None), (prefix_lens, "prefix_lens", ns)))
     if ns == 0 or tq == 0:
         return
-    h, dev = query.size(1), query.device
     mq = min(int(max_q_len), tq)
     mctx = mb * bs if max_context_len is None else min(int(max_context_len), mb * bs)
     need = _scored_ws("npd_paged_prefill_scored_workspace_size", ns, tq, h, kvh, d, mq, mctx)
@@ -1006,8 +1011,8 @@ def paged_prefill_attention_scored(out: torch.Tensor, query: torch.Tensor,
              key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
              cu_seqlens_q.data_ptr(), context_lens.data_ptr(), ns, tq, h, kvh, d, num_blocks, bs,
              mb, mq, mctx, *rule, 0 if first_keys is None else first_keys.data_ptr(),
-             0 if prefix_lens is None else prefix_lens.data_ptr(), *scales, query.stride(0),
-             query.stride(1), out.stride(0), out.stride(1), ws_ptr, ws_bytes, code)
+             0 if prefix_lens is None else prefix_lens.data_ptr(), *scales, *strides, ws_ptr,
+             ws_bytes, code)
 
 
 def _rows_16(*ts: torch.Tensor) -> bool:
@@ -1061,20 +1066,25 @@ def block_norms(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor 
     [rows, width]. 2-byte CUDA tensors of up to 8192 columns run as one launch with
     fp32 inside; others, and calls that record a gradient, as torch operations
     (which refuse what does not fit, or an x that may not be written in place)."""
-    ts = [t for t in (delta, post_weight, weight, x_out) if t is not None]
-    if (x.dim() == 2 and x.size(1) <= 8192 and delta.shape == x.shape and _rows_16(x, *ts)
-            and (post_weight is None or post_weight.shape == x.shape[1:])
-            and (weight is None or weight.shape == x.shape[1:])
-            and (x_out is None or x_out.shape == x.shape)):
+    shape = x.shape
+    if len(shape) == 2 and shape[1] <= 8192 and delta.shape == shape:
+        ts, cols = [x, delta], shape[1:]
+        fits = True
+        for t in (post_weight, weight):
+            if t is not None:
+                fits = fits and t.shape == cols
+                ts.append(t)
+        if x_out is not None:
+            fits = fits and x_out.shape == shape
+            ts.append(x_out)
         strides = (0, 0) if gate is None else _gate_strides(gate, x)
-        if strides is not None:
-            dst = x if x_out is None else x_out
+        if fits and strides is not None and _rows_16(*ts):
             h = None if weight is None else torch.empty_like(x)
-            _call_on(x.device, "npd_block_norms", dst.data_ptr(), 0 if h is None else h.data_ptr(),
-                     x.data_ptr(), delta.data_ptr(),
+            _call_on(x.get_device(), "npd_block_norms", (x if x_out is None else x_out).data_ptr(),
+                     0 if h is None else h.data_ptr(), x.data_ptr(), delta.data_ptr(),
                      0 if post_weight is None else post_weight.data_ptr(),
                      0 if weight is None else weight.data_ptr(),
-                     0 if gate is None else gate.data_ptr(), *strides, x.size(0), x.size(1),
+                     0 if gate is None else gate.data_ptr(), *strides, shape[0], shape[1],
                      float(residual_scale), float(eps), _DTYPES[x.dtype])
             return h
     norm, cols = torch.nn.functional.rms_norm, (x.size(-1),)
