@@ -34,7 +34,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoRef = 3.402823466e38f;   // exponent offset of a row without a reference
 constexpr int kTileRows = 128;              // rows of a workgroup of the rows kernel
 // ... and how many of them run at once on a compute unit at (padded) head dim d
-// (FP8 bytes pass through registers: at three, steps of 128 dims would spill)
+// (FP8 bytes pass through registers: at three, steps of 128 dims spill; 96 tokens in
+// three groups take 130 us, 112 at two)
 __host__ __device__ constexpr int rows_per_cu(int64_t d, bool fp8) {
   return d > 128 ? 1 : d > 64 ? (fp8 ? 2 : 3) : 4;
 }
@@ -78,6 +79,7 @@ struct Args {
   bool list;                      // ... that share the steps of all tiles evenly
   int cost_shift;                 // ... whose cost is counted in 2^shift steps
   int unit_splits;                // stream kernel: most parts of a unit
+  int part_keys;                  // ... fewest keys of one
   int subs, sub_heads;            // stream kernel: units per kv head, heads of a unit
   int window;                     // 0: none
   float scale_log2;               // scale * log2(e)

@@ -6,13 +6,20 @@ namespace npd {
 namespace scored {
 namespace {
 
-constexpr int kTargetItems = 4096;   // waves of a stream launch, about
+constexpr int kOnePart = 256;        // keys up to which a unit is not cut (no merge: 9 us, not 11)
+constexpr int kDecodePart = 64;      // shortest part of a unit that is (keys)
+// Rows of which each has a workgroup to merge it: many parts are then read side by
+// side (64 tokens over 8192 shared keys: 48 us against 51.5; one token of 4000 keys:
+// 13 against 16). More rows fill the chip with a few lanes each.
+constexpr int kWideRows = 2048;
+constexpr int kSharedPart = 256;     // ... beside the rows kernel
 
 template <class TT, int DP, bool kF8>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2)))
 void stream_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) StreamLds<DP> lds;
-  stream_unit<TT, DP, kF8>(a, blockIdx.x, threadIdx.x, lds);
+  constexpr int kRing = DP == 64 || (kF8 && DP == 128) ? 4 : (DP == 128 || kF8 ? 2 : 1);
+  stream_unit<TT, DP, kF8, kRing>(a, blockIdx.x, threadIdx.x, lds);
 }
 
 // Partials of a row: `nt` of its tile (slot t0 and then every second from t1 on,
@@ -87,6 +94,20 @@ __device__ __forceinline__ void tile_parts(const Args& a, int64_t tile, int kh, 
   p.tstep = (int64_t)2 * a.num_kv_heads * kTileRows;
 }
 
+// The parts of one token's row (by a whole wave).
+__device__ __forceinline__ void token_parts(const Args& a, int s, int h, int lane, Parts& p) {
+  int pos, a0, na, b0, nb;
+  unit_keys(a, s, lane, pos, a0, na, b0, nb);
+  p.nu = unit_parts(a, na + nb, lane);
+  p.u0 = ((int64_t)s * a.num_heads + h) * a.unit_splits;
+  Group g;
+  if (a.cu_groups && find_group(a, s, lane, g) && g.shared > 0) {
+    const int kh = h / a.group;
+    const int64_t f = (int64_t)(s - g.seq0) * a.group + (h - kh * a.group);
+    const int64_t tile = g.tile0 + f / kTileRows;
+    if (tile < a.tiles) tile_parts(a, tile, kh, (int)(f % kTileRows), p);
+  }
+}
 // One token per sequence: a wave takes 64 / LPR heads of a token.
 template <class TT, int LPR>
 __global__ __launch_bounds__(256) void merge_tokens_kernel(Args a) {
@@ -96,23 +117,76 @@ __global__ __launch_bounds__(256) void merge_tokens_kernel(Args a) {
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int s = (int)(w / per), h = (int)(w - (int64_t)s * per) * R + lane / LPR;
   if (s >= a.num_seqs) return;   // whole waves
-  int pos, a0, na, b0, nb;
-  unit_keys(a, s, lane, pos, a0, na, b0, nb);
   Parts p{};
-  p.nu = unit_parts(a, na + nb);
-  if (!a.cu_groups && p.nu <= 1) return;   // written by the stream kernel itself
-  Group g;
-  const bool grouped = a.cu_groups && find_group(a, s, lane, g) && g.shared > 0;
-  if (h >= a.num_heads) return;
-  const int kh = h / a.group;
-  p.u0 = ((int64_t)s * a.num_heads + h) * a.unit_splits;
-  if (grouped) {
-    const int64_t f = (int64_t)(s - g.seq0) * a.group + (h - kh * a.group);
-    const int64_t tile = g.tile0 + f / kTileRows;
-    if (tile < a.tiles) tile_parts(a, tile, kh, (int)(f % kTileRows), p);
-  }
+  token_parts(a, s, h < a.num_heads ? h : a.num_heads - 1, lane, p);
+  if (h >= a.num_heads || (!a.cu_groups && p.nu <= 1)) return;   // (one part: written by its unit)
   merge_row<TT, LPR>(a, p, lane, a.out + s * a.out_stride_token + h * a.out_stride_head,
-                     a.v_scale ? a.v_scale[kh] : 1.f);
+                     a.v_scale ? a.v_scale[h / a.group] : 1.f);
+}
+
+// Few rows, or many parts of each: a workgroup per row, its lane groups at a part each.
+template <class TT, int LPR>
+__global__ __launch_bounds__(256) void merge_wide_kernel(Args a) {
+  constexpr int kGroups = 256 / LPR;
+  __shared__ f32x4 s_o[4][LPR];
+  __shared__ float s_l[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = a.head_dim, c = lane % LPR * 4;
+  const int s = blockIdx.x / a.num_heads, h = blockIdx.x - s * a.num_heads;
+  Parts p{};
+  token_parts(a, s, h, lane, p);
+  const int n = p.nt + p.nu;
+  if (!a.cu_groups && n <= 1) return;   // written by its unit
+  auto ml = [&](int i) { return (p.tile(i) ? a.tile_ml : a.unit_ml) + p.slot(i) * 2; };
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 64) M = fmaxf(M, ml(i)[0]);
+  M = wave_max_f(M);
+  f32x4 o = f32x4{0, 0, 0, 0};
+  float L = 0.f;
+  if (M > -INFINITY) {
+    constexpr int kFlight = 4;
+    for (int i0 = threadIdx.x / LPR; i0 < n; i0 += kFlight * kGroups) {
+      float m[kFlight], l[kFlight];
+      f32x4 x[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const int i = i0 + k * kGroups < n ? i0 + k * kGroups : i0;
+        const float* q = ml(i);
+        m[k] = i0 + k * kGroups < n ? q[0] : -INFINITY;
+        l[k] = q[1];
+        x[k] = f32x4{0, 0, 0, 0};
+        if (c < d) x[k] = *reinterpret_cast<const f32x4*>((p.tile(i) ? a.tile_o : a.unit_o) + p.slot(i) * d + c);
+      }
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        // (a part without a key has no sums)
+        const bool has = m[k] != -INFINITY;
+        const float f = __builtin_amdgcn_exp2f(m[k] - M);
+        L = has ? fmaf(l[k], f, L) : L;
+        o.x = has ? fmaf(x[k].x, f, o.x) : o.x;
+        o.y = has ? fmaf(x[k].y, f, o.y) : o.y;
+        o.z = has ? fmaf(x[k].z, f, o.z) : o.z;
+        o.w = has ? fmaf(x[k].w, f, o.w) : o.w;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = LPR; k < 64; k <<= 1) {
+    L += __shfl_xor(L, k, 64);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = o[e];
+      o[e] = v + __shfl_xor(v, k, 64);
+    }
+  }
+  if (lane < LPR) s_o[wave][lane] = o;
+  if (lane == 0) s_l[wave] = L;
+  __syncthreads();
+  if (threadIdx.x >= LPR || c >= d) return;
+  L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  o = (s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane]);
+  const float inv = L > 0.f || L != L ? (a.v_scale ? a.v_scale[h / a.group] : 1.f) / L : 0.f;
+  *reinterpret_cast<u32x2*>(a.out + s * a.out_stride_token + h * a.out_stride_head + c) =
+      u32x2{TT::pack2(o.x * inv, o.y * inv), TT::pack2(o.z * inv, o.w * inv)};
 }
 
 // Chunks: a workgroup takes a tile's rows of one kv head, kSlice of them.
@@ -173,6 +247,8 @@ void launch_merge_d(const Args& a, hipStream_t st) {
   if (a.cu_seqlens_q) {
     const int64_t n = (int64_t)a.tiles * a.num_kv_heads * (kTileRows / kSlice);
     hipLaunchKernelGGL((merge_tiles_kernel<TT, LPR>), dim3((unsigned)n), dim3(256), 0, st, a);
+  } else if ((int64_t)a.num_seqs * a.num_heads <= kWideRows) {
+    hipLaunchKernelGGL((merge_wide_kernel<TT, LPR>), dim3((unsigned)(a.num_seqs * a.num_heads)), dim3(256), 0, st, a);
   } else {
     constexpr int R = 64 / LPR;
     const int64_t waves = (int64_t)a.num_seqs * ((a.num_heads + R - 1) / R);
@@ -193,15 +269,6 @@ void launch_merge(const Args& a, int32_t dtype, hipStream_t st) {
 // Units of at most kUnitHeads heads: the fewest near-equal ones.
 int64_t subs_of(int64_t group) { return (group + kUnitHeads - 1) / kUnitHeads; }
 
-// Most parts of a unit: as many as bring the launch to kTargetItems waves, no
-// more than the table's tokens (or the window's) have parts of kMinPart keys.
-int64_t unit_splits_of(int64_t units, int64_t max_keys) {
-  int64_t w = (kTargetItems + units - 1) / units;
-  const int64_t most = (max_keys + kMinPart - 1) / kMinPart;
-  w = w < most ? w : most;
-  return w < 1 ? 1 : w;
-}
-
 // Workgroups of the rows kernel that run at once per kv head.
 int64_t rows_room(int64_t head_dim, int64_t num_kv_heads, bool fp8) {
   const int64_t n = rows_per_cu(head_dim, fp8) * (int64_t)device_cus() / num_kv_heads;
@@ -215,8 +282,9 @@ int64_t pad256(int64_t x) { return (x + 255) / 256 * 256; }
 // tiles' partials and part counts, then the units'.
 struct Plan {
   int cost_shift = 0;
+  int64_t part_keys = 0;
   int64_t tiles = 0, tiles_max = 0, room = 1, unit_splits = 1;
-  bool list = false;
+  bool list = false, groups = false;
   int64_t tile_slots = 0, unit_slots = 0, head_dim = 0, kv_heads = 0;
   int64_t tile_items_at() const { return kCounterBytes; }
   int64_t tile_o_at() const { return tile_items_at() + (tile_slots ? pad256(tiles * kv_heads * 16) : 0); }
@@ -228,21 +296,38 @@ struct Plan {
   }
 };
 
+// Most parts of a unit: twice what makes kTargetItems waves of units that are all
+// alike, for the longest of a ragged batch; no more than the table's tokens (or the
+// window's) have parts of `least` keys.
+void cut_units(Plan& p, int64_t units, int64_t max_keys, int64_t least) {
+  const int64_t w = max_keys <= kOnePart ? 1 : 2 * ((kTargetItems + units - 1) / units);
+  const int64_t most = (max_keys + least - 1) / least;
+  p.part_keys = least;
+  p.unit_splits = units >= kTargetItems ? 1 : w < most ? w : most;
+  if (p.unit_splits < 1) p.unit_splits = 1;
+}
+
 int64_t window_keys(int64_t max_keys, int64_t window, bool prefix) {
   return window > 0 && !prefix && window < max_keys ? window : max_keys;
 }
 Plan decode_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
-                 int64_t max_keys) {
+                 int64_t max_keys, int64_t least = kDecodePart) {
   Plan p;
   p.head_dim = head_dim;
   p.kv_heads = num_kv_heads;
-  p.unit_splits = unit_splits_of(num_seqs * num_kv_heads * subs_of(num_heads / num_kv_heads), max_keys);
+  cut_units(p, num_seqs * num_kv_heads * subs_of(num_heads / num_kv_heads), max_keys, least);
   p.unit_slots = p.unit_splits > 1 ? num_seqs * num_heads * p.unit_splits : 0;
   return p;
 }
 // Slots of the rows kernel's partials: two per workgroup (its first tile may have
 // begun before it and its last may go on after it); groups also one per tile (the
 // parts of whole tiles meet those of the stream units).
+// Elements of K up to which shared keys are read once per sequence after all: a
+// launch without the rows kernel spares its fixed work, about the time of reading
+// 128 MB. Measured with 4 to 64 sequences, 2 and 8 kv heads, head dims of 64 to 256,
+// once per sequence against shared: at 17 M elements 18 to 24 us against 25 to 35,
+// at 34 M 28 to 34 against 26 to 39, at 67 M 36 to 55 against 28 to 42.
+constexpr int64_t kReadAgain = int64_t(1) << 25;
 // Shares over at most `tiles` tiles of a kv head with at most `steps` steps each.
 void plan_list(Plan& p, int64_t tiles, int64_t steps) {
   const int64_t total = tiles * (steps + kTileCost), most = (total + kMinShare - 1) / kMinShare;
@@ -253,7 +338,10 @@ void plan_list(Plan& p, int64_t tiles, int64_t steps) {
 }
 Plan shared_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                  int64_t max_keys, int64_t num_groups, int64_t max_shared) {
-  Plan p = decode_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_keys);
+  if (num_seqs * num_kv_heads * max_shared <= kReadAgain / head_dim)
+    return decode_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_keys);
+  Plan p = decode_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_keys, kSharedPart);
+  p.groups = true;
   p.unit_slots = num_seqs * num_heads * p.unit_splits;   // always merged
   p.tiles = num_seqs * (num_heads / num_kv_heads) / kTileRows + num_groups;
   p.room = rows_room(head_dim, num_kv_heads, false);
@@ -396,6 +484,7 @@ Args make_args(const Call& c, const Plan& p, void* workspace) {
   a.list = p.list;
   a.cost_shift = p.cost_shift;
   a.unit_splits = (int)p.unit_splits;
+  a.part_keys = (int)p.part_keys;
   a.subs = (int)subs_of(a.group);
   a.sub_heads = (a.group + a.subs - 1) / a.subs;
   a.window = (int)c.window;
@@ -413,6 +502,15 @@ Args make_args(const Call& c, const Plan& p, void* workspace) {
 }
 
 bool grid_ok(int64_t n) { return n <= INT32_MAX; }
+
+int run_decode(const Call& c, const Plan& p, const Args& a, hipStream_t st) {
+  if (!grid_ok(c.num_seqs * c.num_kv_heads * a.subs * p.unit_splits))
+    return fail(NPD_E_INVALID, "%s: too many (seq, kv-head) units", c.name);
+  if (c.dtype == NPD_DTYPE_BF16) launch_stream<BF16>(a, st);
+  else launch_stream<F16>(a, st);
+  if (p.unit_slots) launch_merge(a, c.dtype, st);
+  return check_launch(c.name);
+}
 
 }  // namespace
 }  // namespace scored
@@ -455,13 +553,7 @@ extern "C" int npd_paged_attention_scored(
   Args a = make_args(c, p, workspace);
   a.first_keys = first_keys;
   a.prefix_lens = prefix_lens;
-  if (!grid_ok(num_seqs * num_kv_heads * a.subs * p.unit_splits))
-    return fail(NPD_E_INVALID, "%s: too many (seq, kv-head) units", c.name);
-  hipStream_t st = as_stream(stream);
-  if (dtype == NPD_DTYPE_BF16) launch_stream<BF16>(a, st);
-  else launch_stream<F16>(a, st);
-  if (p.unit_slots) launch_merge(a, dtype, st);
-  return check_launch(c.name);
+  return run_decode(c, p, a, as_stream(stream));
 }
 
 extern "C" int64_t npd_paged_attention_shared_workspace_size(int64_t num_seqs, int64_t num_heads,
@@ -504,6 +596,7 @@ extern "C" int npd_paged_attention_shared(
   rc = check_workspace(c, p, workspace, workspace_bytes);
   if (rc != NPD_OK) return rc;
   Args a = make_args(c, p, workspace);
+  if (!p.groups) return run_decode(c, p, a, as_stream(stream));
   a.cu_groups = cu_groups;
   a.shared_lens = shared_lens;
   a.num_groups = (int)num_groups;

@@ -13,12 +13,17 @@
 // maximum is taken in the usual step. Steps run from the last key back: the
 // newest keys come first, which with a distance term hold the largest scores.
 //
-// What bounds it: the issue of exponentials and reciprocals. One wave issues an
-// exponential every 24 cycles and any other vector instruction every 8 (measured),
-// a SIMD one every 8 and 4: it takes three waves per SIMD to fill it, so registers
-// and LDS are held to three workgroups per compute unit (two at head dims above
-// 128, four up to 64), which run unsynchronised, one's MFMAs under another's
-// exponentials.
+// What bounds it: three things of like size that do not overlap fully. Of a step at
+// 128 dims (128 rows by 32 keys) a compute unit's MFMAs take 0.22 us, the issue of a
+// capped softmax 0.25 (per score two exponentials or reciprocals and one more, 8
+// cycles an instruction, others 4; both together, measured in registers alone, 0.31)
+// and the LDS reads of K and V operands, 64 KB, 0.21; in place a step takes 0.6.
+// Workgroups of one compute unit run unsynchronised, one's waits under another's
+// issue: three (168 registers, operands read two ahead of their MFMA) take 1359 us
+// over 12000 tokens of 32 / 8 heads of 128, capped (868 TFLOP/s of the 1263 that a
+// large matrix product reaches), two 1436. At 256 dims one workgroup has the unit:
+// for two, 200 bytes of registers spill within the loop (packed documents: 221 us
+// against 130).
 //
 // Masked keys: P is 0 by selection, but 0 times an infinity or NaN in V is NaN,
 // and rows of a tile do not see the same keys. So a row whose result is not
@@ -28,7 +33,10 @@
 // Shares: where whole tiles would leave the chip uneven, its workgroups take equal
 // shares of all tiles' steps, laid end to end (rows_share), from the lengths on the
 // device. A share may end one tile, hold whole ones and begin another; the pieces
-// of a tile meet in the merge kernel.
+// of a tile meet in the merge kernel. A piece costs 10 to 13 us besides its steps
+// (finding it 4, its rows and ranges 4, its list of blocks 1.4, the first tiles 2,
+// storing 2.5), a step 0.65 us of a compute unit. Chunks of 300 to 512 tokens over
+// 3000, shared out: 112 us; cut into equal parts of each tile: 122.
 #pragma once
 
 #include "scored_stream.h"
@@ -833,7 +841,8 @@ void shared_kernel(Args a) {
     rows_group<TT, D, kF8, kCapped, kBias>(blockIdx.x, lds.rows);
   } else {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    stream_unit<TT, D, kF8>(a, ((int)blockIdx.x - n) * (kThreads / 64) + wave, threadIdx.x & 63,
+    constexpr int kRing = D == 64 || (kF8 && D == 128) ? 4 : (D == 128 || kF8 ? 2 : 1);
+    stream_unit<TT, D, kF8, kRing>(a, ((int)blockIdx.x - n) * (kThreads / 64) + wave, threadIdx.x & 63,
                             lds.stream[wave]);
   }
 }

@@ -11,11 +11,15 @@
 //   the head's reference moves only when a step's maximum passes it by 2^8;
 //   O^T += V^T . P^T on v_mfma_f32_16x16x16, V through LDS for the transposing
 //     reads of its operand.
-// Loads run kRing steps ahead in registers (about 16 KB of a wave in flight at
-// any head dim). Bound: HBM, the unit's K/V bytes.
-// Parts: a unit's keys are cut into near-equal parts of at least kMinPart keys,
-// as many as the launch has waves for it (unit_splits), from the lengths on the
-// device; the parts meet in the merge kernel.
+// Loads run kRing steps ahead in registers (8 to 16 KB of a wave in flight).
+// Bound: HBM, the units' K/V bytes (64 sequences of 128 to 4096 keys, 32 / 8 heads of
+// 128, bf16: 117 us, 4.83 TB/s of the 4.92 that a large copy reaches). Short ones
+// are bound by the chain length -> table -> K -> step, 9 us a call with its launch.
+// Parts: a unit's keys are cut into near-equal parts, from the lengths on the device
+// (part_len); the parts meet in a merge kernel. At 1000 and 4000 keys of one
+// sequence, parts of 64 keys take 11 and 13 us where parts of 256 take 22 and 27;
+// four deep rings of 128 dims (64 KB in flight) took 5% longer over full batches,
+// and at 256 dims spill.
 #pragma once
 
 #include "scored.h"
@@ -23,8 +27,13 @@
 namespace npd {
 namespace scored {
 
+// Waves of a stream launch, about: what keeps HBM busy at any raggedness. Parts
+// shorter than kLongPart keys spend more on their start and merge than they spare
+// once there are kFewItems of them.
+constexpr int kTargetItems = 4096;
+constexpr int kFewItems = 1024;
+constexpr int kLongPart = 256;
 constexpr int kListKeys = 1024;      // rows listed in LDS at a time (a multiple of every ring)
-constexpr int kMinPart = 256;        // shortest part of a unit (keys)
 constexpr float kTau = 8.f;          // a reference moves by more than this (log2 units)
 
 // Nontemporal: a pool row is read once per call (by one unit per kv head).
@@ -57,8 +66,27 @@ __device__ __forceinline__ void unit_keys(const Args& a, int s, int lane, int& p
   na = ae > a0 ? ae - a0 : 0;
   // prefix keys past the token: none (pre <= context = position + 1)
 }
-__device__ __forceinline__ int unit_parts(const Args& a, int keys) {
-  const int p = (keys + kMinPart - 1) / kMinPart;
+// Keys of a part, of one length for all units: beside the rows kernel and for units
+// that are not cut the host's, else what makes kTargetItems parts (or kFewItems
+// shorter ones) of all keys (of each stride-th sequence, where there are many).
+__device__ __forceinline__ int part_len(const Args& a, int lane) {
+  if (a.cu_groups || a.unit_splits == 1) return a.part_keys;
+  const int stride = (a.num_seqs + 511) / 512;
+  float sum = 0.f;
+  for (int s = lane * stride; s < a.num_seqs; s += 64 * stride) {
+    const int ctx = clampi(a.seq_lens[s], 0, a.max_bps * a.block_size);
+    const Keys k = row_keys(ctx - 1, ctx, a.first_keys ? a.first_keys[s] : 0,
+                            a.prefix_lens ? a.prefix_lens[s] : 0, a.window);
+    sum += (float)(k.hi - k.lo) + (float)max(0, min(k.pre, k.lo) - k.first);
+  }
+  const float total = wave_sum_f(sum) * (float)(a.num_kv_heads * a.subs * stride);
+  const int few = (int)fminf(total * (1.f / kFewItems), 1e9f);
+  const int n = (int)fminf(total * (1.f / kTargetItems), 1e9f);
+  return max(a.part_keys, (max(n, min(few, kLongPart)) + 15) / 16 * 16);
+}
+__device__ __forceinline__ int unit_parts(const Args& a, int keys, int lane) {
+  const int len = part_len(a, lane);
+  const int p = keys / len + (keys % len != 0);
   return p < a.unit_splits ? p : a.unit_splits;
 }
 
@@ -70,9 +98,8 @@ struct StreamLds {
   uint16_t v[16 * (DP + 16)];      // rows of DP + 16 elements: an 8-bank shift per row
   int row[kListKeys];
 };
-template <class TT, int DP, bool kF8>
+template <class TT, int DP, bool kF8, int kRing>
 __device__ __forceinline__ void stream_unit(const Args& a, int item, int lane, StreamLds<DP>& lds) {
-  constexpr int kRing = DP == 64 || (kF8 && DP == 128) ? 4 : (DP == 128 || kF8 ? 2 : 1);
   constexpr int EB = kF8 ? 1 : 2;                  // bytes per element
   constexpr int CPR = DP * EB / 16;                // 16-byte chunks per (padded) row
   constexpr int NKL = CPR / 4;                     // K loads per lane and step
@@ -97,7 +124,7 @@ __device__ __forceinline__ void stream_unit(const Args& a, int item, int lane, S
   int pos, a0, na, b0, nb;
   unit_keys(a, s, lane, pos, a0, na, b0, nb);
   const int keys = na + nb;
-  const int parts = unit_parts(a, keys);
+  const int parts = unit_parts(a, keys, lane);
   const bool direct = !a.cu_groups && parts <= 1;
   uint16_t* orow = a.out + s * a.out_stride_token + (h0 + n16) * a.out_stride_head;
   if (part >= parts) {
