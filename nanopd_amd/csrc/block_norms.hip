@@ -9,7 +9,8 @@
 //
 // Bound by HBM bytes at many rows (x and delta read, x_out and h written, each
 // once: the row stays in registers between the two statistics), by the latency
-// of load, two reductions and store at few.
+// of load, two reductions and store at few. 16384 rows of 5120, gated per row:
+// 128 us, 5.2 TB/s; 527 of 4096: 5.5 us, 3.2 TB/s; one row of 4096: 3.3 us.
 #include "common.h"
 
 namespace {

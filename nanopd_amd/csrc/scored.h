@@ -72,7 +72,7 @@ struct Args {
   int num_seqs, num_groups, total_q, max_shared;
   int num_heads, num_kv_heads, group, head_dim;
   int block_size, bs_shift, num_blocks, max_bps;   // bs_shift < 0: no power of two
-  int tiles;                      // rows kernel: tiles of all sequences or groups
+  int tiles;                      // rows kernel: tiles of all groups, or tiles_max of each sequence
   int tiles_max;                  // ... chunks: most tiles of one sequence
   int room;                       // ... workgroups per kv head (chunks without a list: whole tiles)
   int room1;                      // ... of them in one round over the compute units

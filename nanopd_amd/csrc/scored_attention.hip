@@ -198,31 +198,20 @@ __global__ __launch_bounds__(256) void merge_tiles_kernel(Args a) {
   const int slice = id % (kTileRows / kSlice);
   id /= kTileRows / kSlice;
   const int kh = id % a.num_kv_heads;
-  const int64_t tile = id / a.num_kv_heads;
-  // the sequence: the last whose first tile is at or before this one
-  auto first = [&](int s) {
-    return (int64_t)clampi(a.cu_seqlens_q[s], 0, a.total_q) * a.group / kTileRows + s;
-  };
-  int lo = 0, hi = a.num_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first(mid) <= tile) lo = mid; else hi = mid - 1;
-  }
-  const int q0 = clampi(a.cu_seqlens_q[lo], 0, a.total_q);
-  const int q1 = clampi(a.cu_seqlens_q[lo + 1], q0, a.total_q);
-  const int64_t t = tile - first(lo);
-  const int64_t rows = (int64_t)(q1 - q0) * a.group;
-  if (t < 0 || t >= a.tiles_max || t * kTileRows >= rows) return;
+  const int tile = id / a.num_kv_heads, sq = tile / a.tiles_max, t = tile - sq * a.tiles_max;
+  const int q0 = clampi(a.cu_seqlens_q[sq], 0, a.total_q);
+  const int q1 = clampi(a.cu_seqlens_q[sq + 1], q0, a.total_q);
+  const int rows = (q1 - q0) * a.group;
+  if (t * kTileRows >= rows) return;
   const float oscale = a.v_scale ? a.v_scale[kh] : 1.f;
   for (int r = slice * kSlice + threadIdx.x / LPR; r < (slice + 1) * kSlice; r += 256 / LPR) {
-    const int64_t f = t * kTileRows + r;
+    const int f = t * kTileRows + r;
     if (f >= rows) break;
     Parts p{};
     tile_parts(a, tile, kh, r, p);
     if (p.nt <= 1) return;     // written by the rows kernel itself
-    const int64_t tok = f / a.group;
-    const int h = kh * a.group + (int)(f - tok * a.group);
-    merge_row<TT, LPR>(a, p, lane, a.out + (q0 + tok) * a.out_stride_token + h * a.out_stride_head,
+    const int tok = f / a.group, h = kh * a.group + (f - tok * a.group);
+    merge_row<TT, LPR>(a, p, lane, a.out + (int64_t)(q0 + tok) * a.out_stride_token + h * a.out_stride_head,
                        oscale);
   }
 }
@@ -355,13 +344,14 @@ Plan chunk_plan(int64_t num_seqs, int64_t total_q, int64_t num_heads, int64_t nu
   const int64_t g = num_heads / num_kv_heads;
   p.head_dim = head_dim;
   p.kv_heads = num_kv_heads;
-  p.tiles = total_q * g / kTileRows + num_seqs;
   p.tiles_max = (max_q_len * g + kTileRows - 1) / kTileRows;
   p.room = rows_room(head_dim, num_kv_heads, false);
-  const int64_t all = num_seqs * p.tiles_max, most = p.tiles < all ? p.tiles : all;
+  const int64_t all = num_seqs * p.tiles_max, rows = total_q * g / kTileRows + num_seqs;
+  const int64_t most = rows < all ? rows : all;
   // shared out evenly unless whole tiles fill the chip twice over
   if (all <= kListTiles && most < 2 * p.room) {
-    plan_list(p, most, max_keys / kStepKeys + 2);
+    p.tiles = all;
+    plan_list(p, all, max_keys / kStepKeys + 2);
     p.tile_slots = p.room > 1 ? 2 * p.room * num_kv_heads * kTileRows : 0;
   } else {
     p.room = all;

@@ -215,7 +215,7 @@ __device__ __forceinline__ void rows_share(const Args& a, int id, int done, int 
       bool ok = true;
       if (chunks) {
         chunk(pc.s, pc.row0, pc.tokens, pc.limit);
-        pc.tile = (int)((int64_t)pc.row0 * G / kTileRows) + pc.s + pc.t;
+        pc.tile = pc.s * a.tiles_max + pc.t;
       } else {
         Group r;
         ok = find_group(a, pc.s, lane, r) && r.tile0 + pc.t < a.tiles;   // (not: groups that overlap)

@@ -394,6 +394,20 @@ def test_chunks_of_every_count(device, d, heads):
         check_prefill(b, q[:n], out[:n], some, d ** -0.5, 40.0, None, 0, None, None)
 
 
+def test_padded_buffers(device):
+    """A batch in a much longer buffer, whose rows past the last sequence stay, and
+    sequences without a token between others."""
+    b = Batch(device, [700, 90, 33], 2, 64, 16, BF16, seed=20)
+    n = 40000
+    q = torch.zeros(n, 8, 64, dtype=BF16, device=device)
+    q[:150] = b.queries(150, 8)
+    out = torch.full_like(q, 7.0)
+    pk.paged_prefill_attention_scored(out, q, b.kc, b.vc, b.table, cu_of([100, 50, 0], device),
+                                      b.seq_lens(), 0.1, 16, b.table.size(1), 100, softcap=9.0)
+    check_prefill(b, q[:150], out[:150], [(100, 600), (50, 40), (0, 33)], 0.1, 9.0, None, 0, None, None)
+    assert (out[150:] == 7.0).all()
+
+
 def test_max_context_len_bounds_only_the_plan(device):
     b = Batch(device, [700, 90], 2, 64, 16, BF16, seed=16)
     q = b.queries(150, 8)
