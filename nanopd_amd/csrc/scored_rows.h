@@ -693,19 +693,33 @@ __device__ __forceinline__ void rows_piece(const Args& a, const Piece& it, int i
   uint16_t* op = a.out + dst.strides(a.out_stride_token, a.out_stride_head);
   if (dst.ok && !((bad_rows >> c) & 1)) {
     const float inv = ltot > 0.f ? oscale / ltot : 0.f;
+    if (merged) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int e = db * 32 + i * 8 + hf * 4;
-        if (e >= d) continue;
-        const f32x4 v = f32x4{oacc[db][4 * i], oacc[db][4 * i + 1], oacc[db][4 * i + 2], oacc[db][4 * i + 3]};
-        if (merged)
-          *reinterpret_cast<f32x4*>(a.tile_o + (slot0 + c) * d + e) = v;
-        else
-          *reinterpret_cast<u32x2*>(op + e) =
-              u32x2{TT::pack2(v.x * inv, v.y * inv), TT::pack2(v.z * inv, v.w * inv)};
-      }
+        for (int i = 0; i < 4; ++i) {
+          const int e = db * 32 + i * 8 + hf * 4;
+          if (e >= d) continue;
+          *reinterpret_cast<f32x4*>(a.tile_o + (slot0 + c) * d + e) =
+              f32x4{oacc[db][4 * i], oacc[db][4 * i + 1], oacc[db][4 * i + 2], oacc[db][4 * i + 3]};
+        }
+    } else {
+      // of 16 dims the lane has 4 hf .. + 3 and 8 + 4 hf ..; the other half of the wave,
+      // which holds the same row, gives it those that make eight in a row
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const int e = db * 32 + i * 8 + hf * 8;
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = TT::pack2(oacc[db][4 * i + 2 * k] * inv, oacc[db][4 * i + 2 * k + 1] * inv);
+          const auto p = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+          const auto q = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+          if (e < d) *reinterpret_cast<u32x4*>(op + e) = u32x4{p[0], q[0], p[1], q[1]};
+        }
+    }
     if (merged && hf == 0) {
       a.tile_ml[(slot0 + c) * 2] = nmref == kNoRef ? -INFINITY : -nmref;
       a.tile_ml[(slot0 + c) * 2 + 1] = ltot;

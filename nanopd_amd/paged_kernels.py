@@ -752,17 +752,19 @@ def _score_rule(what, out, query, key_cache, value_cache, block_tables, seqs, sc
         _fp8_cache_checks(key_cache, value_cache, k_scale, v_scale)
         if k_scale.get_device() != dev or v_scale.get_device() != dev:
             _fail(f"k_scale and v_scale must be on {query.device}")
-    else:
+    elif (key_cache.dim() != 4 or value_cache.shape != key_cache.shape
+          or key_cache.dtype is not dtype or value_cache.dtype is not dtype
+          or not key_cache.is_contiguous() or not value_cache.is_contiguous()):
         _cache_checks(key_cache, value_cache)
-        if key_cache.dtype is not dtype:
-            _fail("query/cache dtype mismatch")
+        _fail("query/cache dtype mismatch")
     for t in (out, key_cache, value_cache):
         if t.get_device() != dev:
             _fail(f"tensor on {t.device}, expected {query.device}")
     for t, nm, least in lens:
         if t is None and nm in _optional:
             continue
-        _int32(t, nm)
+        if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32):
+            _int32(t, nm)
         if (t.get_device() != dev or t.dim() != 1 or t.numel() < (n if least is None else least)
                 or not t.is_contiguous()):
             _fail(f"{nm} must be a contiguous int32 vector of at least {n if least is None else least} "
@@ -1066,26 +1068,29 @@ def block_norms(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor 
     [rows, width]. 2-byte CUDA tensors of up to 8192 columns run as one launch with
     fp32 inside; others, and calls that record a gradient, as torch operations
     (which refuse what does not fit, or an x that may not be written in place)."""
-    shape = x.shape
-    if len(shape) == 2 and shape[1] <= 8192 and delta.shape == shape:
-        ts, cols = [x, delta], shape[1:]
-        fits = True
-        for t in (post_weight, weight):
-            if t is not None:
-                fits = fits and t.shape == cols
-                ts.append(t)
-        if x_out is not None:
-            fits = fits and x_out.shape == shape
-            ts.append(x_out)
+    shape, dtype = x.shape, x.dtype
+    if (len(shape) == 2 and 0 < shape[1] <= 8192 and not shape[1] & 7 and shape[0] and x.is_cuda
+            and delta.shape == shape and dtype in _DTYPES):
+        # what the kernel reads as it is: whole 16-byte rows of one dtype and one GPU
+        cols, dev, grad = shape[1:], x.get_device(), torch.is_grad_enabled()
+        ptrs, fits = [], True
+        for t, want in ((x, shape), (delta, shape), (post_weight, cols), (weight, cols),
+                        (x_out, shape)):
+            if t is None:
+                ptrs.append(0)
+                continue
+            ptr = t.data_ptr()
+            ptrs.append(ptr)
+            if (t.shape != want or t.dtype is not dtype or ptr & 15 or t.get_device() != dev
+                    or not t.is_contiguous() or (grad and t.requires_grad)):
+                fits = False
+                break
         strides = (0, 0) if gate is None else _gate_strides(gate, x)
-        if fits and strides is not None and _rows_16(*ts):
+        if fits and strides is not None:
             h = None if weight is None else torch.empty_like(x)
-            _call_on(x.get_device(), "npd_block_norms", (x if x_out is None else x_out).data_ptr(),
-                     0 if h is None else h.data_ptr(), x.data_ptr(), delta.data_ptr(),
-                     0 if post_weight is None else post_weight.data_ptr(),
-                     0 if weight is None else weight.data_ptr(),
-                     0 if gate is None else gate.data_ptr(), *strides, shape[0], shape[1],
-                     float(residual_scale), float(eps), _DTYPES[x.dtype])
+            _call_on(dev, "npd_block_norms", ptrs[4] or ptrs[0], 0 if h is None else h.data_ptr(),
+                     ptrs[0], ptrs[1], ptrs[2], ptrs[3], 0 if gate is None else gate.data_ptr(),
+                     *strides, shape[0], shape[1], float(residual_scale), float(eps), _DTYPES[dtype])
             return h
     norm, cols = torch.nn.functional.rms_norm, (x.size(-1),)
     d = delta.float()
