@@ -470,7 +470,7 @@ int npd_paged_attention_scored(void* out, const void* query,
  * npd_paged_attention_scored of a batch whose sequences share prefixes (no
  * reference counterpart; its block manager's fork shares the blocks,
  * nanoPD/block_manager/block_manager.py:100-105): the same result, each shared
- * key read once per group. Group g < num_groups: the sequences cu_groups[g] ..
+ * key read once per group (or, where there are few, once per sequence). Group g < num_groups: the sequences cu_groups[g] ..
  * cu_groups[g+1] - 1 (cu_groups: int32 [num_groups + 1], ascending), whose
  * tables hold the same blocks for their first shared_lens[g] keys (the first
  * sequence's table is read there). A sequence shorter than that sees its own

@@ -270,7 +270,6 @@ int64_t pad256(int64_t x) { return (x + 255) / 256 * 256; }
 // ops leave alone, so that one buffer serves every attention op), then the
 // tiles' partials and part counts, then the units'.
 struct Plan {
-  int cost_shift = 0;
   int64_t part_keys = 0;
   int64_t tiles = 0, tiles_max = 0, room = 1, unit_splits = 1;
   bool list = false, groups = false;
@@ -322,11 +321,10 @@ void plan_list(Plan& p, int64_t tiles, int64_t steps) {
   const int64_t total = tiles * (steps + kTileCost), most = (total + kMinShare - 1) / kMinShare;
   p.list = true;
   p.room = p.room < most ? p.room : most < 1 ? 1 : most;
-  while (p.cost_shift < 30 && ((steps + kTileCost) >> p.cost_shift) + 1 > (INT32_MAX / 2) / tiles)
-    ++p.cost_shift;
 }
 Plan shared_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                  int64_t max_keys, int64_t num_groups, int64_t max_shared) {
+  max_shared = max_shared < max_keys ? max_shared : max_keys;
   if (num_seqs * num_kv_heads * max_shared <= kReadAgain / head_dim)
     return decode_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_keys);
   Plan p = decode_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_keys, kSharedPart);
@@ -472,7 +470,11 @@ Args make_args(const Call& c, const Plan& p, void* workspace) {
   }
   a.room1 = (int)((device_cus() + c.num_kv_heads - 1) / c.num_kv_heads);
   a.list = p.list;
-  a.cost_shift = p.cost_shift;
+  // (units in which all tiles' costs stay below 2^30, whatever the lengths)
+  if (p.list)
+    while (a.cost_shift < 30 &&
+           ((c.block_size * c.max_bps / kStepKeys + kTileCost) >> a.cost_shift) + 1 > (INT32_MAX / 2) / p.tiles)
+      ++a.cost_shift;
   a.unit_splits = (int)p.unit_splits;
   a.part_keys = (int)p.part_keys;
   a.subs = (int)subs_of(a.group);

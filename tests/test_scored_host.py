@@ -212,7 +212,8 @@ def test_c_entries_refuse_their_own():
         assert c_shared(**change) == INVALID and b"groups" in err()
     assert c_shared(cu=None) == INVALID and c_shared(sh=None) == INVALID and b"null" in err()
     # (as many groups as there can be: their costs are counted in coarser steps)
-    assert c_shared(g=2 ** 31 - 1, msh=4096) == WORKSPACE
+    assert c_shared(g=2 ** 31 - 1, msh=4096, s=3000, mb=2 ** 20) == WORKSPACE
+    assert c_shared(msh=2 ** 62, s=3000) == WORKSPACE
     assert c_prefill(cu=None) == INVALID and b"null" in err()
     for change in (dict(mq=0), dict(mq=2 ** 31), dict(mc=-1)):
         assert c_prefill(**change) == INVALID and b"max_q_len" in err()
@@ -252,6 +253,9 @@ def test_workspace_sizes():
     assert pk.scored_workspace_bytes(4, 32, 8, 128, 16, 512, window=128) == 0
     assert pk.scored_workspace_bytes(4, 32, 8, 128, 16, 512, window=128, prefix=True) == a
     assert pk.shared_workspace_bytes(4, 32, 8, 128, 16, 512, 1, 4096) > 0
+    # shared keys are counted to the table's end
+    assert pk.shared_workspace_bytes(64, 32, 8, 128, 16, 512, 1, 2 ** 62) == \
+        pk.shared_workspace_bytes(64, 32, 8, 128, 16, 512, 1, 8192)
     assert pk.prefill_scored_workspace_bytes(1, 40000, 32, 8, 128, 40000, 40000) == 0   # whole tiles
     assert pk.prefill_scored_workspace_bytes(2, 600, 32, 8, 128, 300, 4000) > 0
     for bad in ((0, 8, 2, 64, 16, 4), (4, 8, 2, 64, 16, 2 ** 31), (2 ** 31, 8, 2, 64, 16, 4)):
