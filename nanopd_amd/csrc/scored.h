@@ -39,6 +39,10 @@ constexpr int kTileRows = 128;              // rows of a workgroup of the rows k
 __host__ __device__ constexpr int rows_per_cu(int64_t d, bool fp8) {
   return d > 128 ? 1 : d > 64 ? (fp8 ? 2 : 3) : 4;
 }
+// Waves of the stream kernel on a SIMD at (padded) head dim d, by its registers.
+__host__ __device__ constexpr int stream_per_simd(int64_t d, bool fp8) {
+  return d > 128 ? 2 : d > 64 ? (fp8 ? 2 : 3) : (fp8 ? 4 : 3);
+}
 constexpr int kStepKeys = 32;               // keys per step of the rows kernel
 // Shares of the rows kernel's workgroups, in steps: what a piece of a tile costs
 // besides its steps, the smallest share (but for its tilt), and how near a tile's edge no cut is made.
@@ -80,6 +84,7 @@ struct Args {
   int cost_shift;                 // ... whose cost is counted in 2^shift steps
   int unit_splits;                // stream kernel: most parts of a unit
   int part_keys;                  // ... fewest keys of one
+  float stream_waves;             // ... waves that run at once
   int subs, sub_heads;            // stream kernel: units per kv head, heads of a unit
   int window;                     // 0: none
   float scale_log2;               // scale * log2(e)

@@ -15,7 +15,7 @@ constexpr int kWideRows = 2048;
 constexpr int kSharedPart = 256;     // ... beside the rows kernel
 
 template <class TT, int DP, bool kF8>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(stream_per_simd(DP, kF8))))
 void stream_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) StreamLds<DP> lds;
   constexpr int kRing = DP == 64 || (kF8 && DP == 128) ? 4 : (DP == 128 || kF8 ? 2 : 1);
@@ -477,6 +477,7 @@ Args make_args(const Call& c, const Plan& p, void* workspace) {
       ++a.cost_shift;
   a.unit_splits = (int)p.unit_splits;
   a.part_keys = (int)p.part_keys;
+  a.stream_waves = (float)(stream_per_simd(c.head_dim, c.k_scale != nullptr) * 4 * device_cus());
   a.subs = (int)subs_of(a.group);
   a.sub_heads = (a.group + a.subs - 1) / a.subs;
   a.window = (int)c.window;

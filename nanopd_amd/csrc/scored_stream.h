@@ -27,9 +27,12 @@
 namespace npd {
 namespace scored {
 
-// Waves of a stream launch, about: what keeps HBM busy at any raggedness. Parts
-// shorter than kLongPart keys spend more on their start and merge than they spare
-// once there are kFewItems of them.
+// Waves of a stream launch, about: for ragged lengths several rounds of them, for
+// lengths within a quarter of their mean the one round that runs at once (40 tokens
+// with 4160 keys each in a window, FP8: 75 us against 92; 64 of 4000: 101 against
+// 115; ragged to 4000 or 16000 one round takes 85 against 77 and 183 against 156).
+// Parts shorter than kLongPart keys spend more on their start and merge than they
+// spare once there are kFewItems of them.
 constexpr int kTargetItems = 4096;
 constexpr int kFewItems = 1024;
 constexpr int kLongPart = 256;
@@ -67,21 +70,32 @@ __device__ __forceinline__ void unit_keys(const Args& a, int s, int lane, int& p
   // prefix keys past the token: none (pre <= context = position + 1)
 }
 // Keys of a part, of one length for all units: beside the rows kernel and for units
-// that are not cut the host's, else what makes kTargetItems parts (or kFewItems
-// shorter ones) of all keys (of each stride-th sequence, where there are many).
+// that are not cut the host's, else by all keys (of each stride-th sequence, where
+// there are many) over the waves wanted.
+// (The merge comes to the same length: no operation may be contracted in one of them.)
 __device__ __forceinline__ int part_len(const Args& a, int lane) {
+#pragma clang fp contract(off)
   if (a.cu_groups || a.unit_splits == 1) return a.part_keys;
   const int stride = (a.num_seqs + 511) / 512;
-  float sum = 0.f;
+  float sum = 0.f, most = 0.f, count = 0.f;
   for (int s = lane * stride; s < a.num_seqs; s += 64 * stride) {
     const int ctx = clampi(a.seq_lens[s], 0, a.max_bps * a.block_size);
     const Keys k = row_keys(ctx - 1, ctx, a.first_keys ? a.first_keys[s] : 0,
                             a.prefix_lens ? a.prefix_lens[s] : 0, a.window);
-    sum += (float)(k.hi - k.lo) + (float)max(0, min(k.pre, k.lo) - k.first);
+    const float keys = (float)(k.hi - k.lo) + (float)max(0, min(k.pre, k.lo) - k.first);
+    sum += keys;
+    most = fmaxf(most, keys);
+    count += 1.f;
   }
-  const float total = wave_sum_f(sum) * (float)(a.num_kv_heads * a.subs * stride);
+  sum = wave_sum_f(sum);
+  count = wave_sum_f(count);
+  const float units = (float)(a.num_kv_heads * a.subs), total = sum * units * (float)stride;
+  // one round of even lengths: each unit's last part is half a part long on average
+  const bool even = wave_max_f(most) * count <= 1.25f * sum;
+  const float items = even ? fmaxf(a.stream_waves - 0.5f * units * (float)a.num_seqs, 0.5f * a.stream_waves)
+                           : (float)kTargetItems;
   const int few = (int)fminf(total * (1.f / kFewItems), 1e9f);
-  const int n = (int)fminf(total * (1.f / kTargetItems), 1e9f);
+  const int n = (int)fminf(total / items, 1e9f);
   return max(a.part_keys, (max(n, min(few, kLongPart)) + 15) / 16 * 16);
 }
 __device__ __forceinline__ int unit_parts(const Args& a, int keys, int lane) {

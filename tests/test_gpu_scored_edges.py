@@ -301,6 +301,20 @@ def test_results_repeat_bit_for_bit(device):
         assert all(torch.equal(x, y) for x, y in zip(o, first))
 
 
+@pytest.mark.parametrize("lens", [
+    [400 + (37 * i) % 90 for i in range(700)],               # more than are counted, even
+    [(131 * i) % 1500 for i in range(600)],                  # ragged
+    [0] * 5 + [3000] + [1] * 9, [0] * 8, [5000], [257, 256, 255, 64, 65],
+], ids=range(6))
+def test_parts_of_many_lengths(device, lens):
+    b = Batch(device, lens, 1, 64, 16, F16, seed=21)
+    q = b.queries(len(lens), 4)
+    out = torch.full_like(q, float("nan"))
+    pk.paged_attention_scored(out, q, b.kc, b.vc, b.table, b.seq_lens(), 0.1, 16, b.table.size(1),
+                              softcap=15.0)
+    check_decode(b, q, out, 0.1, 15.0, None, 0, None, None)
+
+
 # -- groups ---------------------------------------------------------------------------------
 
 def shared_case(device, lens, groups, kvh=2, heads=8, d=64, seed=12, max_shared=None, tables=None):
